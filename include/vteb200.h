@@ -315,6 +315,87 @@ int vteb_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_ca
                          const int* kv_offsets, int batch, int num_kv_heads, int head_dim,
                          long long kv_batch_stride, void* stream);
 
+/* ---- paged caches --------------------------------------------------------
+ * A cache as a pool of pages of `page_size` positions (16, 32, 64 or 128).  A block table int32[batch, max_pages] says
+ * which pages hold a sequence's positions, in order; kv_offsets int32[batch] is the position of its newest token, as for
+ * the contiguous caches, and -1 where a row of the batch is padding.  All of them are device memory; entries of the table
+ * behind a sequence's last page are not read.  No counterpart in the reference.
+ *
+ * Types of the pages.  VTEB_PAGED_F16 holds fp16.  VTEB_PAGED_E4M3 and VTEB_PAGED_INT8 hold 8-bit values with one fp32
+ * scale for every page and KV head, of K and of V (k_scale, v_scale fp32[num_pages, num_kv_heads]): a stored value stands
+ * for value * scale.  vteb_paged_append keeps the scale at the largest magnitude of the page over 448 (e4m3) or 127
+ * (int8): tokens that join a page only ever raise it, and then the page's older tokens are rounded anew under the new
+ * scale; the token of a page's first position starts the page afresh.  A value that is not finite makes the scale NaN.
+ * vteb_paged_attention takes any scales.
+ *
+ * Layout.  Position t of KV head h of page p starts page_stride * p + head_stride * h + token_stride * t values into the
+ * pool, head_dim (64, 128 or 256) values side by side; strides are multiples of 16 bytes and rows do not overlap.  With
+ * the positions of a head side by side (head_stride = page_size * head_dim) a page's part is one run of memory, which
+ * DRAM serves best; heads side by side (token_stride = num_kv_heads * head_dim) is the contiguous cache's order. */
+#define VTEB_PAGED_F16 0
+#define VTEB_PAGED_E4M3 1
+#define VTEB_PAGED_INT8 2
+#define VTEB_PAGED_MAX_QUERY_TOKENS 16
+#define VTEB_PAGED_MAX_POSITIONS (1 << 30)   /* max_pages * page_size */
+typedef struct vteb_paged_cache_t {
+    void* k_pool;
+    void* v_pool;
+    float* k_scale;            /* null for fp16 pages */
+    float* v_scale;
+    long long page_stride, token_stride, head_stride;   /* values */
+    int num_pages, page_size, num_kv_heads, head_dim, type;
+    int ready;                 /* set by vteb_paged_cache_init */
+    unsigned char maps[256];   /* the pools' tensor maps, likewise */
+} vteb_paged_cache_t;
+/* Checks the fields in front of `ready` and sets the others.  Once for a pool; nothing is kept outside the structure. */
+int vteb_paged_cache_init(vteb_paged_cache_t* cache);
+
+/* New tokens of each sequence into its pages, K rotated to its positions on the way and, with q, the queries of the same
+ * tokens rotated into q_out (which may be q).  k, v [total_tokens, num_kv_heads, head_dim] and q, q_out [total_tokens,
+ * num_q_heads, head_dim] fp16, the heads of a token side by side, tokens at the strides given (halves, multiples of 8: k, v
+ * and q may be parts of one projection's rows).  The tokens of sequence b are rows token_starts[b] to token_starts[b + 1] -
+ * 1 (int32[batch + 1], device), or total_tokens / batch rows each where token_starts is null; the last of them has
+ * position kv_offsets[b], so tokens at positions below 0 are padding and neither stored nor rotated.  kv_offsets is the array that the attention behind takes.
+ * Rotation: rope_type -1 none, 0 / 1 / 2 and the fp16 tables [rope_rows, head_dim or rotary_dim] as for rope_kernel
+ * (rotary_dim a multiple of 16).  Two tokens of one call must not have the same place, and with 8-bit pages a page that is
+ * appended to must be one sequence's.  What lies behind the newest token of a page is left as it is.
+ * status (may be null): int that a kernel sets to 5 where a table entry lies outside the pool and to 6 where a
+ * position lies beyond the block table or the rotation tables; such tokens are not stored. */
+typedef struct vteb_paged_append_t {
+    const void *k, *v, *q;     /* q and q_out null: no queries */
+    void* q_out;
+    long long k_token_stride, v_token_stride, q_token_stride, q_out_token_stride;
+    const int *block_table, *kv_offsets, *token_starts;
+    const void *rope_cos, *rope_sin;
+    int* status;
+    int batch, max_pages, total_tokens, num_q_heads;
+    int rope_type, rotary_dim, rope_rows;
+} vteb_paged_append_t;
+int vteb_paged_append(const vteb_paged_cache_t* cache, const vteb_paged_append_t* args, void* stream);
+
+/* Attention of the newest query_tokens (1 to 16) tokens of each sequence over its cached positions, one launch.
+ * q and output [batch, query_tokens, num_q_heads, head_dim] contiguous, q fp16, output fp16 or fp32 (out_is_f32); query
+ * token i of sequence b sees positions 0..kv_offsets[b] - query_tokens + 1 + i.  A row that sees nothing is zero, and its
+ * lse (fp32[batch, query_tokens, num_q_heads], natural log, may be null) -infinity.  Positions that a row does not see do
+ * not reach it, whatever they hold.  The result is the same bits for the same inputs.
+ * workspace: vteb_paged_attention_workspace bytes, 256-byte aligned, zeroed before its first use (each call leaves it ready
+ * for the next).  Calls that share one must not overlap on the GPU, whatever their shapes.
+ * status as above, and 1 where a bounded wait ran out; the rows of a sequence with a table entry outside the pool are NaN,
+ * and a kv_offset beyond the table stands for the table's last position. */
+typedef struct vteb_paged_attention_t {
+    const void* q;
+    void* output;
+    float* lse;
+    const int *block_table, *kv_offsets;
+    void* workspace;
+    size_t workspace_bytes;
+    int* status;
+    float scale;
+    int out_is_f32, batch, max_pages, num_q_heads, query_tokens;
+} vteb_paged_attention_t;
+int vteb_paged_attention_workspace(int num_q_heads, int num_kv_heads, int head_dim, int batch, int query_tokens, size_t* bytes);
+int vteb_paged_attention(const vteb_paged_cache_t* cache, const vteb_paged_attention_t* args, void* stream);
+
 /* Reads the status word a split kernel leaves in work[1] and clears it.
  * Returns VTEB_ERR_DEVICE_STATUS when a bounded wait gave up. */
 int vteb_check_status(int* work, void* stream);

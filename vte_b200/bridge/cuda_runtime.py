@@ -103,6 +103,29 @@ class HostStep(ctypes.Structure):
                 ("q_bytes", ctypes.c_size_t), ("out_bytes", ctypes.c_size_t), ("batch", ctypes.c_int), ("capacity", ctypes.c_int)]
 
 
+class PagedCache(ctypes.Structure):
+    """Mirror of `vteb_paged_cache_t` (include/vteb200.h)."""
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("k_pool", "v_pool", "k_scale", "v_scale")] +
+                [(name, ctypes.c_longlong) for name in ("page_stride", "token_stride", "head_stride")] +
+                [(name, ctypes.c_int) for name in ("num_pages", "page_size", "num_kv_heads", "head_dim", "type", "ready")] +
+                [("maps", ctypes.c_ubyte * 256)])
+
+
+class PagedAppend(ctypes.Structure):
+    """Mirror of `vteb_paged_append_t` (include/vteb200.h)."""
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("k", "v", "q", "q_out")] +
+                [(name, ctypes.c_longlong) for name in ("k_token_stride", "v_token_stride", "q_token_stride", "q_out_token_stride")] +
+                [(name, ctypes.c_void_p) for name in ("block_table", "kv_offsets", "token_starts", "rope_cos", "rope_sin", "status")] +
+                [(name, ctypes.c_int) for name in ("batch", "max_pages", "total_tokens", "num_q_heads", "rope_type", "rotary_dim", "rope_rows")])
+
+
+class PagedAttention(ctypes.Structure):
+    """Mirror of `vteb_paged_attention_t` (include/vteb200.h)."""
+    _fields_ = ([(name, ctypes.c_void_p) for name in ("q", "output", "lse", "block_table", "kv_offsets", "workspace")] +
+                [("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p), ("scale", ctypes.c_float)] +
+                [(name, ctypes.c_int) for name in ("out_is_f32", "batch", "max_pages", "num_q_heads", "query_tokens")])
+
+
 class ClusterGrid(tuple):
     """Grid dimensions of a launch whose blocks form thread-block clusters of `cluster` along x."""
     def __new__(cls, dims, cluster: int):
@@ -189,6 +212,10 @@ def _declare(lib):
         "vteb_check_status": (i, [vp, vp]),
         "vteb_noalloc_check_status": (i, [vp]),
         "vteb_module_check_status": (i, [vp]),
+        "vteb_paged_cache_init": (i, [ctypes.POINTER(PagedCache)]),
+        "vteb_paged_append": (i, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedAppend), vp]),
+        "vteb_paged_attention_workspace": (i, [i, i, i, i, i, szp]),
+        "vteb_paged_attention": (i, [ctypes.POINTER(PagedCache), ctypes.POINTER(PagedAttention), vp]),
         "vteb_fill_normal_f16": (i, [vp, sz, ull, f, f, f, vp]),
         "vteb_read_bandwidth_probe": (i, [vp, sz, vp, i, vp]),
     }
@@ -706,7 +733,8 @@ class CudaRuntime:
         """Raise, once, if a launch that has completed gave up on a bounded wait and its arguments name no status word."""
         if self._launch_status is not None and self._launch_status.value:
             code, self._launch_status.value = self._launch_status.value, 0
-            raise CudaRuntimeError(f"a kernel gave up on a bounded wait (code {code})", code=ERR_DEVICE_STATUS)
+            what = {5: "a block table names a page outside the pool", 6: "a position lies beyond its block table or rotation tables"}
+            raise CudaRuntimeError(f"{what.get(code, 'a kernel gave up on a bounded wait')} (code {code})", code=ERR_DEVICE_STATUS)
 
     def module_check_status(self, module) -> None:
         """Raise, once, if a launch of a loaded module's cluster kernels with a null status gave up.  Waits for the device."""
@@ -920,6 +948,46 @@ class CudaRuntime:
         if err < 0:
             raise CudaSafetyError(f"vteb_kv_cache_append refused the call ({err}): {self._last_error()}")
         self._check_error(err, "vteb_kv_cache_append")
+
+    def paged_cache_init(self, cache: PagedCache) -> None:
+        """Checks a paged cache's fields and encodes its tensor maps into it."""
+        self._require_init()
+        self._check_paged(self._lib.vteb_paged_cache_init(ctypes.byref(cache)), "vteb_paged_cache_init")
+
+    def paged_attention_workspace(self, num_q_heads: int, num_kv_heads: int, head_dim: int, batch: int, query_tokens: int = 1) -> int:
+        """Bytes of scratch that a call of `paged_attention` needs, zeroed before its first use."""
+        self._require_init()
+        n = ctypes.c_size_t(0)
+        self._check_paged(self._lib.vteb_paged_attention_workspace(num_q_heads, num_kv_heads, head_dim, batch, query_tokens, ctypes.byref(n)),
+                          "vteb_paged_attention_workspace")
+        return n.value
+
+    def paged_append(self, cache: PagedCache, args: PagedAppend, stream: Optional[int] = None) -> None:
+        """New tokens into their pages, on `stream` (a CUDA stream's address) or the runtime's own.  Where `args.status` is
+        null, bad pages and positions are reported by the runtime's next wait."""
+        self._paged_call(self._lib.vteb_paged_append, cache, args, stream)
+
+    def paged_attention(self, cache: PagedCache, args: PagedAttention, stream: Optional[int] = None) -> None:
+        """The newest tokens' attention over a paged cache, on `stream` or the runtime's own; status as for `paged_append`."""
+        self._paged_call(self._lib.vteb_paged_attention, cache, args, stream)
+
+    def _paged_call(self, call, cache, args, stream) -> None:
+        self._require_init()
+        if self._panic:
+            raise CudaSafetyError("runtime is in panic state (a synchronize timed out); new launches are blocked")
+        named = args.status
+        if not named:
+            args.status = ctypes.addressof(self._launch_status)
+        err = call(cache, args, self._stream if stream is None else stream)
+        if not named:
+            args.status = None
+        if err:
+            self._check_paged(err, call.__name__)
+
+    def _check_paged(self, err: int, what: str) -> None:
+        if err < 0:
+            raise CudaSafetyError(f"{what} refused the call ({err}): {self._last_error()}")
+        self._check_error(err, what)
 
     def check_status(self, work) -> None:
         """Raise if a split kernel recorded a timed-out wait in work[1]."""

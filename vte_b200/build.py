@@ -33,12 +33,13 @@ def _newer(target: Path, sources) -> bool:
 
 
 def build_library(force: bool = False, verbose: bool = False) -> Path:
-    sources = [CSRC / "vteb200_shim.cu", *sorted(CSRC.glob("*.h")), *sorted((CSRC / "kernels").glob("*.cu*")),
+    units = [CSRC / "vteb200_shim.cu", CSRC / "vteb200_paged.cu"]
+    sources = [*units, *sorted(CSRC.glob("*.h")), *sorted((CSRC / "kernels").glob("*.cu*")),
                PKG.parent / "include" / "vteb200.h"]
     if not force and _newer(LIB, sources):
         return LIB
     cmd = [_nvcc(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-diag-suppress", "550", "-o", str(LIB), str(CSRC / "vteb200_shim.cu"), "-ldl"]
+           "-diag-suppress", "550", "--threads", str(len(units)), "-o", str(LIB), *map(str, units), "-ldl"]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd))

@@ -1,3 +1,4 @@
+from .paged_cache import PagedKVCache
 from .split_kv_attention import SplitKVAttentionDispatcher
 
-__all__ = ["SplitKVAttentionDispatcher"]
+__all__ = ["PagedKVCache", "SplitKVAttentionDispatcher"]

@@ -12,6 +12,7 @@
 
 #include "../../include/vteb200.h"
 #include "cluster_choice.h"
+#include "shim_internal.h"
 #include "kernels/decode_attention.cu"
 #include "kernels/aux_kernels.cu"
 
@@ -188,6 +189,32 @@ int launch_rt(void (*kernel)(Args...), dim3 grid, dim3 block, size_t smem, cudaS
 }
 
 }  // namespace
+
+namespace vteb_shim {
+
+int report(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+int report_rt(cudaError_t e, const char* what) { return check_rt(e, what); }
+int report_drv(CUresult r, const char* what) { return check_drv(r, what); }
+int device_index() { return g_initialized ? g_device : -1; }
+
+int encode_tiled(CUtensorMap* map, CUtensorMapDataType type, cuuint32_t rank, void* base, const cuuint64_t* dims,
+                 const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+    const int rc = driver_api();
+    if (rc) return rc;
+    const cuuint32_t ones[5] = {1u, 1u, 1u, 1u, 1u};
+    return check_drv(g_drv.TensorMapEncodeTiled(map, type, rank, base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                                                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+                     "cuTensorMapEncodeTiled");
+}
+
+}  // namespace vteb_shim
 
 extern "C" {
 
