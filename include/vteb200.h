@@ -370,6 +370,7 @@ typedef struct vteb_paged_append_t {
     int* status;
     int batch, max_pages, total_tokens, num_q_heads;
     int rope_type, rotary_dim, rope_rows;
+    int launch_flags;          /* VTEB_LAUNCH_PROGRAMMATIC or 0 */
 } vteb_paged_append_t;
 int vteb_paged_append(const vteb_paged_cache_t* cache, const vteb_paged_append_t* args, void* stream);
 
@@ -392,6 +393,7 @@ typedef struct vteb_paged_attention_t {
     int* status;
     float scale;
     int out_is_f32, batch, max_pages, num_q_heads, query_tokens;
+    int launch_flags;          /* as above */
 } vteb_paged_attention_t;
 int vteb_paged_attention_workspace(int num_q_heads, int num_kv_heads, int head_dim, int batch, int query_tokens, size_t* bytes);
 int vteb_paged_attention(const vteb_paged_cache_t* cache, const vteb_paged_attention_t* args, void* stream);

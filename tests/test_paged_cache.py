@@ -179,38 +179,36 @@ def test_e4m3_grid_and_rounding():
     assert orc.to_e4m3(np.float32(1e9)) == 126 and orc.to_e4m3(np.float32(np.nan)) & 127 == 127
 
 
-def worker_runs(lengths, head_rows, unit, grid, gw):
-    """The runs of units that paged_attention_kernel deals to its workers, as (workers, total, [(lo, hi)])."""
-    total = sum(-(-n // unit) for n in lengths) * head_rows
-    workers = min(grid * (8 // gw), max(1, -(-total // (2 * gw))))
-    return workers, total, [(w * total // workers, (w + 1) * total // workers) for w in range(workers)]
+def worker_runs(lengths, head_rows, unit, grid, groups, warps):
+    """The runs of units that paged_attention_kernel deals to its workers, as (units of a run, total, [(lo, hi)])."""
+    total = sum(-(-int(n) // unit) for n in lengths) * head_rows
+    per = max(-(-total // (grid * groups)), 2 * (warps // groups))
+    return per, total, [(lo, min(lo + per, total)) for lo in range(0, total, per)]
 
 
-@pytest.mark.parametrize("gw", [1, 2, 4, 8])
-def test_pieces_of_cut_segments_have_places_of_their_own(gw):
+@pytest.mark.parametrize("groups", [1, 2, 4, 8, 16])
+def test_pieces_of_cut_segments_have_places_of_their_own(groups):
     """The kernel's arithmetic for segments that worker borders cut: first and last worker, the piece each one leaves and the
     counter they share."""
-    rng = np.random.default_rng(gw)
+    rng = np.random.default_rng(groups)
     for _ in range(60):
         lengths = rng.integers(0, rng.choice([40, 500, 9000]), size=rng.integers(1, 40))
         head_rows, unit = int(rng.choice([1, 2, 8])), int(rng.choice([16, 32, 64]))
-        workers, total, runs = worker_runs(lengths, head_rows, unit, 148, gw)
-        if not total:
-            continue
-        assert runs[0][0] == 0 and runs[-1][1] == total and all(a[1] == b[0] and a[0] < a[1] for a, b in zip(runs, runs[1:] + [(total, 0)]))
+        per, total, runs = worker_runs(lengths, head_rows, unit, 148, groups, 16)
+        assert len(runs) <= 148 * groups and all(lo < hi for lo, hi in runs)
         begin, pieces, counters = 0, set(), set()
         for n in lengths:
             for _ in range(head_rows if n else 0):
                 units = -(-int(n) // unit)
                 owners = [w for w, (lo, hi) in enumerate(runs) if lo < begin + units and hi > begin]
-                w0, w1 = ((begin + 1) * workers - 1) // total, ((begin + units) * workers - 1) // total
+                w0, w1 = begin // per, (begin + units - 1) // per
                 assert owners == list(range(w0, w1 + 1))
                 if len(owners) > 1:
                     assert w0 not in counters
                     counters.add(w0)
                     for k, w in enumerate(owners):
                         place = 2 * w + (0 if runs[w][0] >= begin else 1)          # as the worker writes it
-                        assert place == (2 * w0 + (0 if runs[w0][0] == begin else 1) if k == 0 else 2 * w)   # as it is read
+                        assert place == (2 * w0 + (0 if w0 * per == begin else 1) if k == 0 else 2 * w)   # as it is read
                         assert place not in pieces
                         pieces.add(place)
                 begin += units

@@ -116,14 +116,14 @@ class PagedAppend(ctypes.Structure):
     _fields_ = ([(name, ctypes.c_void_p) for name in ("k", "v", "q", "q_out")] +
                 [(name, ctypes.c_longlong) for name in ("k_token_stride", "v_token_stride", "q_token_stride", "q_out_token_stride")] +
                 [(name, ctypes.c_void_p) for name in ("block_table", "kv_offsets", "token_starts", "rope_cos", "rope_sin", "status")] +
-                [(name, ctypes.c_int) for name in ("batch", "max_pages", "total_tokens", "num_q_heads", "rope_type", "rotary_dim", "rope_rows")])
+                [(name, ctypes.c_int) for name in ("batch", "max_pages", "total_tokens", "num_q_heads", "rope_type", "rotary_dim", "rope_rows", "launch_flags")])
 
 
 class PagedAttention(ctypes.Structure):
     """Mirror of `vteb_paged_attention_t` (include/vteb200.h)."""
     _fields_ = ([(name, ctypes.c_void_p) for name in ("q", "output", "lse", "block_table", "kv_offsets", "workspace")] +
                 [("workspace_bytes", ctypes.c_size_t), ("status", ctypes.c_void_p), ("scale", ctypes.c_float)] +
-                [(name, ctypes.c_int) for name in ("out_is_f32", "batch", "max_pages", "num_q_heads", "query_tokens")])
+                [(name, ctypes.c_int) for name in ("out_is_f32", "batch", "max_pages", "num_q_heads", "query_tokens", "launch_flags")])
 
 
 class ClusterGrid(tuple):

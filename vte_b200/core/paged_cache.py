@@ -18,7 +18,7 @@ from __future__ import annotations
 import ctypes
 import math
 
-from ..bridge.cuda_runtime import PagedAppend, PagedAttention, PagedCache, _ptr_value
+from ..bridge.cuda_runtime import LAUNCH_PROGRAMMATIC, PagedAppend, PagedAttention, PagedCache, _ptr_value
 from ..bridge.errors import CudaSafetyError
 from ..bridge.memory import MemoryRegion
 
@@ -82,6 +82,7 @@ class PagedKVCache:
         self._append = PagedAppend(num_q_heads=self.num_q_heads, rope_type=-1, k_token_stride=kv_row, v_token_stride=kv_row,
                                    q_token_stride=q_row, q_out_token_stride=q_row)
         self._attention = PagedAttention(num_q_heads=self.num_q_heads)
+        self._append.launch_flags = self._attention.launch_flags = 0 if getattr(hip, '_no_pdl', True) else LAUNCH_PROGRAMMATIC
         self._default_strides = (kv_row, kv_row, q_row, q_row)
         self._default_scale = 1.0 / math.sqrt(self.head_dim)
 

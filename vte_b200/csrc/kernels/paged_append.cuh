@@ -135,6 +135,9 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
 {
     const int D = 1 << p.dim_log2, tasks_log2 = p.dim_log2 - 4, P = 1 << p.page_log2;
     const int tid = threadIdx.x, T = blockDim.x;
+    // nothing of the launches in front is touched before this; the launch behind may start when they are complete
+    grid_dependency_wait();
+    grid_launch_dependents();
     if ((int)blockIdx.x >= p.kv_blocks) {                   // ---- Q
         const long long all = ((long long)p.total_tokens * p.num_q_heads) << tasks_log2;
         const long long t0 = (long long)(blockIdx.x - p.kv_blocks) * T * kAppendQTasks + tid;

@@ -8,8 +8,8 @@
 //
 // Work.  The positions of a sequence are cut into units of U positions (4 to 8 KB of K and as much of V); (sequence, KV
 // head, block of rows) is a segment, and all units of all segments, in that order, are dealt as equal runs to the
-// workers.  A worker is `gw` of the eight warps of a CTA: the runs and `gw` are computed on the device from the step's
-// own lengths.  Each warp of a worker takes every gw-th unit and has a ring of its own in shared memory, which its own
+// workers.  A worker is `gw` of the warps of a CTA, one CTA an SM: the runs and `gw` are computed on the device from the
+// step's own lengths.  Each warp of a worker takes every gw-th unit and has a ring of its own in shared memory, which its own
 // lanes fill with tensor-map copies (one box a page) and which only it reads: no warp waits for another between the
 // ends of segments, and the loads of the next segment are in flight while one is merged.
 //
@@ -26,6 +26,8 @@
 // who is last.
 #pragma once
 
+#include <type_traits>
+
 #include "vteb_common.cuh"
 
 namespace vteb {
@@ -33,10 +35,6 @@ namespace vteb {
 constexpr int kPagedF16 = 0, kPagedE4m3 = 1, kPagedInt8 = 2;
 constexpr int kStatusBadPage = 5;        // a block table entry outside 0..num_pages-1 for a position that is read or written
 constexpr int kStatusBadPosition = 6;    // a position beyond the block table or the rotation tables
-
-constexpr int kPagedWarps = 8;
-constexpr int kPagedThreads = kPagedWarps * 32;
-constexpr int kPagedRing = 24 * 1024;    // bytes of a warp's ring
 
 struct PagedAttnArgs {
     KvTensorMap k_map, v_map;
@@ -53,33 +51,34 @@ struct PagedAttnArgs {
     int* status;
     int batch, max_pages, num_pages, page_log2, box_log2;
     int num_q_heads, num_kv_heads, group, queries, row_blocks;
+    unsigned group_inv;              // ceil(2^31 / group): r / group = 2 r * group_inv >> 32 for the 2^16 rows r there can be
     float scale_log2e;
 };
 
-template <int D, int KIND>
+// Positions of a unit (4 or 8 KB of K, and as much of V) and warps of a CTA, so that the rings (192 KB of an SM's 227) hold at
+// least two units a warp and a thread's accumulators, Q fragments and scores fit its registers (168 with 12 warps).
+__host__ __device__ constexpr int paged_unit(int row_bytes) { return row_bytes >= 256 ? 16 : 4096 / row_bytes; }
+__host__ __device__ constexpr int paged_warps(int row_bytes, int head_dim, int nt) {
+    return row_bytes == 512 ? 6 : head_dim * nt == 256 ? 8 : 12;
+}
+
+template <int D, int KIND, int NT>
 struct PagedShape {
     static constexpr int ES = KIND == kPagedF16 ? 2 : 1;
     static constexpr int RB = D * ES;                       // bytes of a row
     static constexpr int CB = RB < 128 ? RB : 128;          // bytes of a column block: the width of a box
-    static constexpr int NC = RB / CB;
-    static constexpr int U = RB == 64 ? 64 : RB <= 256 ? 32 : 16;      // positions of a unit
-    static constexpr int SLOT = U * RB;
-    static constexpr int NS = kPagedRing / SLOT;            // slots of a ring: K, V, K, V, ...
-    static constexpr int MAXBOX = U / 16;
-};
-
-template <int NT> struct PagedMerge {                       // cross-warp merge, DC columns at a time
+    static constexpr int W = paged_warps(RB, D, NT);
+    static constexpr int RING = 192 * 1024 / W;             // bytes of a warp's ring
+    static constexpr int U = paged_unit(RB);                           // positions of a unit
+    static constexpr int SLOT = 2 * U * RB;                 // K, then V
+    static constexpr int NS = RING / SLOT;
     static constexpr int ROWS = 8 * NT;
-    static constexpr int DC = NT == 1 ? 64 : 32;
-    static constexpr int LD = DC + 4;                       // rows 2i, 2i+1 of a fragment land on different banks
-    static constexpr int WARP_FLOATS = ROWS * LD;
+    static constexpr int PART = 1024;                       // bytes a warp has for the last merge's parts, and for the newest tokens' weights
+    static constexpr int SMEM = 1024 + W * (RING + PART + ROWS * 8 + 4 * 4 * 8 + 64);
+    static_assert(NS >= 2 && NS <= 4, "units in a ring");
+    static_assert(ROWS * D * 4 <= SLOT, "a warp's rows fit the slot that it read last");
+    static_assert(PART >= 32 * 24 && PART >= 15 * ROWS * 4, "parts and weights");
 };
-
-template <int NT>
-__host__ __device__ constexpr int paged_smem_bytes() {
-    // rings, merge buffers, per warp: (m, l) of its rows, scales of its slots, barriers
-    return 1024 + kPagedWarps * (kPagedRing + PagedMerge<NT>::WARP_FLOATS * 4 + 8 * NT * 8 + 8 * 16 + 8 * 8);
-}
 
 #if defined(__CUDACC__)
 
@@ -88,6 +87,12 @@ __device__ __forceinline__ void tma_load_pages(uint32_t dst, const void* map, in
         "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
         ::"r"(dst), "l"(map), "r"(0), "r"(y), "r"(0), "r"(head), "r"(page), "r"(bar)
         : "memory");
+}
+
+__device__ __forceinline__ bool elect_one() {               // true in one lane of a warp, always the same one
+    uint32_t yes;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes != 0;
 }
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -102,7 +107,7 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     return y;
 }
 
-// Four 8-bit values to fp16, exactly: lo = values 0 and 1 of the word (2 and 3 with them in hi), or with `pairs` 0 and 2
+// Four 8-bit values to fp16, exactly: lo = values 0 and 1 of the word (2 and 3 with them in hi), or with `PAIRS` 0 and 2
 // (1 and 3), which is how ldmatrix.trans leaves two positions of two channels.
 template <int KIND, bool PAIRS>
 __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -123,13 +128,11 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) {
     }
 }
 
-// Byte offset inside a box of BR rows (column blocks one after another, swizzled) of 16-byte chunk `chunk` of row `r`.
+// Byte offset inside a box (column blocks of `block` bytes one after another, swizzled) of 16-byte chunk `chunk` of row `r`.
 template <int CB>
-__device__ __forceinline__ uint32_t box_offset(int r, int chunk, int box_rows) {
+__device__ __forceinline__ uint32_t box_offset(int r, int chunk, int block) {
     constexpr int PER = CB / 16;                            // chunks of a column block
-    const int cb = chunk / PER, c = chunk % PER;
-    const int x = CB == 128 ? (c ^ (r & 7)) : (c ^ ((r >> 1) & 3));
-    return (uint32_t)(cb * box_rows * CB + r * CB + x * 16);
+    return (uint32_t)((chunk / PER) * block + r * CB + (((chunk % PER) ^ (CB == 128 ? r & 7 : (r >> 1) & 3)) * 16));
 }
 
 __device__ __forceinline__ void group_barrier(int gw, int group) {
@@ -137,27 +140,26 @@ __device__ __forceinline__ void group_barrier(int gw, int group) {
     else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(gw * 32) : "memory");
 }
 
-// Where a warp is in its worker's run: unit `u` of segment (b, hr), of which units [first, end) are this worker's.
+// Where a warp is in its worker's run: unit `u` of a segment, of which units [first, end) are this worker's.
 struct PagedCursor {
-    int b, hr, u, first, end, units, len;
-    long long left;                                         // units of the run from `first` on
+    int b, head, rb, u, first, end, units, len;
+    int left;                                               // units of the run from `first` on
 };
 
 __device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) {
-    const int room = a.max_pages << a.page_log2;            // at most 2^31 - 1, checked by the host
+    const int room = a.max_pages << a.page_log2;            // at most 2^30, checked by the host
     const int off = __ldg(a.kv_offsets + b);
     return off < 0 ? 0 : off >= room ? room : off + 1;
 }
 
 template <int U>
-__device__ __forceinline__ void cursor_enter(const PagedAttnArgs& a, PagedCursor& c) {   // first segment at or behind (b, hr) that has units
+__device__ __forceinline__ void cursor_enter(const PagedAttnArgs& a, PagedCursor& c) {   // first sequence at or behind c.b that has units
     c.len = paged_len(a, c.b);
     c.units = (c.len + U - 1) / U;
     while (c.units == 0 && c.b + 1 < a.batch) {
         c.len = paged_len(a, ++c.b);
         c.units = (c.len + U - 1) / U;
     }
-    c.end = (long long)(c.units - c.first) < c.left ? c.units : c.first + (int)c.left;
 }
 
 template <int U>
@@ -165,308 +167,310 @@ __device__ __forceinline__ bool cursor_next_segment(const PagedAttnArgs& a, Page
     c.left -= c.end - c.first;
     if (c.left <= 0) return false;
     c.first = 0;
-    if (++c.hr == a.num_kv_heads * a.row_blocks) {
-        c.hr = 0;
-        ++c.b;
-        cursor_enter<U>(a, c);
-    } else {
-        c.end = (long long)c.units < c.left ? c.units : (int)c.left;
+    if (++c.rb == a.row_blocks) {
+        c.rb = 0;
+        if (++c.head == a.num_kv_heads) {
+            c.head = 0;
+            ++c.b;
+            cursor_enter<U>(a, c);
+        }
     }
-    return true;
+    c.end = min(c.units, c.left);
+    return c.units > 0;                                     // (no units left: lengths that changed under the launch)
 }
 
 template <int D, int KIND, int NT, bool F32>
-__global__ void __launch_bounds__(kPagedThreads, 1) paged_attention_kernel(const __grid_constant__ PagedAttnArgs a)
+__global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_attention_kernel(const __grid_constant__ PagedAttnArgs a)
 {
-    using S = PagedShape<D, KIND>;
-    using M = PagedMerge<NT>;
-    constexpr int U = S::U, RB = S::RB, CB = S::CB, NS = S::NS, SLABS = U / 16, KSTEPS = D / 16, ROWS = 8 * NT;
+    using S = PagedShape<D, KIND, NT>;
+    constexpr int U = S::U, RB = S::RB, CB = S::CB, NS = S::NS, W = S::W, SLABS = U / 16, KSTEPS = D / 16, ROWS = S::ROWS;
     constexpr bool kScaled = KIND != kPagedF16;
 
     extern __shared__ unsigned char smem_raw[];
-    __shared__ long long s_scan[kPagedWarps];
-    __shared__ int s_live[kPagedWarps];
-    __shared__ int s_start_b[kPagedWarps];
-    __shared__ long long s_start_rest[kPagedWarps];
-    __shared__ int s_last[kPagedWarps];
-    __shared__ float s_denom[kPagedWarps][ROWS];            // of the rows of each worker's segment
+    __shared__ int s_scan[W], s_live[W], s_start_b[W], s_start_rest[W], s_last[W], s_slot[W];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    unsigned char* ring = smem + warp * kPagedRing;
-    float* merge_all = reinterpret_cast<float*>(smem + kPagedWarps * kPagedRing);
-    float2* ml_all = reinterpret_cast<float2*>(merge_all + kPagedWarps * M::WARP_FLOATS);
-    float* scales = reinterpret_cast<float*>(ml_all + kPagedWarps * ROWS) + warp * 32;         // [slot][4]
-    unsigned long long* bars = reinterpret_cast<unsigned long long*>(reinterpret_cast<float*>(ml_all + kPagedWarps * ROWS) + kPagedWarps * 32) + warp * 8;
+    unsigned char* ring = smem + warp * S::RING;
+    unsigned char* part_all = smem + W * S::RING;
+    float2* ml_all = reinterpret_cast<float2*>(part_all + W * S::PART);
+    float2* scales = ml_all + W * ROWS + warp * 16;                                           // [unit % 4][box], of K and V
+    unsigned long long* bars = reinterpret_cast<unsigned long long*>(ml_all + W * ROWS + W * 16) + warp * 8;
     const uint32_t ring_u = smem_u32(ring), bars_u = smem_u32(bars), scales_u = smem_u32(scales);
+
+    if (lane == 0) {
+        for (int i = 0; i < NS; ++i) mbar_init(bars_u + i * 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (warp == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&a.k_map) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&a.v_map) : "memory");
+        }
+    }
+    // nothing of the launches in front is touched before this; the launch behind may start when they are complete
+    grid_dependency_wait();
+    grid_launch_dependents();
 
     const int box_rows = 1 << a.box_log2;
     const int boxes = U >> a.box_log2;                      // of a unit
-    if (lane == 0) {
-        for (int i = 0; i < NS; ++i) mbar_init(bars_u + i * 8, 1 + (kScaled ? boxes : 0));
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
+    const int HR = a.num_kv_heads * a.row_blocks;
 
     // ---- all units, and where this CTA's workers begin ------------------------------------------
-    const int HR = a.num_kv_heads * a.row_blocks;
-    const int per_thread = (a.batch + kPagedThreads - 1) / kPagedThreads;
-    const int b0 = min(tid * per_thread, a.batch), b1 = min(b0 + per_thread, a.batch);
-    long long mine = 0;
-    int live = 0;
-    for (int b = b0; b < b1; ++b) {
-        const int units = (paged_len(a, b) + U - 1) / U;
-        mine += units;
-        live += units > 0;
-        if (blockIdx.x == 0 && a.status && __ldg(a.kv_offsets + b) >= (a.max_pages << a.page_log2)) *a.status = kStatusBadPosition;
-    }
-    long long upto = mine;
-    int live_upto = live;
+    int total, lives, mine = 0, upto = 0, b0 = 0, b1 = 1;
+    if (a.batch == 1) {
+        total = (paged_len(a, 0) + U - 1) / U;
+        lives = total > 0;
+        __syncwarp();
+    } else {
+        const int per_thread = (a.batch + W * 32 - 1) / (W * 32);
+        b0 = min(tid * per_thread, a.batch);
+        b1 = min(b0 + per_thread, a.batch);
+        int live = 0;
+        for (int b = b0; b < b1; ++b) {
+            const int units = (paged_len(a, b) + U - 1) / U;
+            mine += units;
+            live += units > 0;
+        }
+        upto = mine;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long x = __shfl_up_sync(~0u, upto, d);
-        const int y = __shfl_up_sync(~0u, live_upto, d);
-        if (lane >= d) { upto += x; live_upto += y; }
-    }
-    if (lane == 31) { s_scan[warp] = upto; s_live[warp] = live_upto; }
-    __syncthreads();
-    long long total = 0;
-    int lives = 0;
+        for (int d = 1; d < 32; d <<= 1) {
+            const int x = __shfl_up_sync(~0u, upto, d);
+            if (lane >= d) upto += x;
+        }
+        live = __reduce_add_sync(~0u, live);
+        if (lane == 31) { s_scan[warp] = upto; s_live[warp] = live; }
+        __syncthreads();
+        total = lives = 0;
 #pragma unroll
-    for (int w = 0; w < kPagedWarps; ++w) {
-        if (w < warp) upto += s_scan[w];
-        total += s_scan[w];
-        lives += s_live[w];
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) upto += s_scan[w];
+            total += s_scan[w];
+            lives += s_live[w];
+        }
     }
     total *= HR;
-    // Warps of a worker.
-    const long long segments = (long long)lives * HR;
-    int gw = kPagedWarps;
-    while (gw > 1 && segments * 4 >= (long long)gridDim.x * (kPagedWarps / gw) * 2 &&
-           (total >= (long long)gridDim.x * (kPagedWarps / gw) * 2 * 16 || total < segments * gw)) gw >>= 1;
-    const int groups = kPagedWarps / gw, group = warp / gw, wi = warp % gw;
-    long long workers = (long long)gridDim.x * groups;
-    const long long useful = (total + 2 * gw - 1) / (2 * gw);
-    if (workers > useful) workers = useful > 0 ? useful : 1;
+    // Workers of a CTA.
+    const int segments = lives * HR, grid = gridDim.x;
+    int groups = 1;
+    while (groups < W) {                                    // 1, 2, 4, 12 or 1, 2, 4, 8 or 1, 2, 6
+        const int more = W % 8 && groups * 4 > W ? W : groups * 2;
+        if (segments * 4 < grid * more || (total < grid * more * 16 && total >= segments * (W / more) * 2)) break;
+        groups = more;
+    }
+    const int gw = W / groups, group = groups == 1 ? 0 : warp / gw, wi = groups == 1 ? warp : warp - group * gw;
+    const int per = max((total + grid * groups - 1) / (grid * groups), gw);              // units of a worker
     const int worker = blockIdx.x * groups + group;
-    for (int g = 0; g < groups; ++g) {
-        const long long w = (long long)blockIdx.x * groups + g;
-        if (w >= workers) break;
-        const long long lo = w * total / workers;
-        if (lo >= (upto - mine) * HR && lo < upto * HR) {
-            long long rest = lo - (upto - mine) * HR;
-            int b = b0;
-            for (; b < b1; ++b) {
-                const long long n = (long long)((paged_len(a, b) + U - 1) / U) * HR;
-                if (rest < n) break;
-                rest -= n;
+    const int lo = worker * per, hi = min(lo + per, total);
+    if (a.batch > 1) {
+        for (int g = 0; g < groups; ++g) {
+            const int at = (blockIdx.x * groups + g) * per;
+            if (at >= (upto - mine) * HR && at < upto * HR) {
+                int rest = at - (upto - mine) * HR, b = b0;
+                for (; b < b1; ++b) {
+                    const int n = (paged_len(a, b) + U - 1) / U * HR;
+                    if (rest < n) break;
+                    rest -= n;
+                }
+                s_start_b[g] = b;
+                s_start_rest[g] = rest;
             }
-            s_start_b[g] = b;
-            s_start_rest[g] = rest;
         }
+        __syncthreads();
     }
-    __syncthreads();
 
-    // ---- sequences without positions: zero rows ---------------------------------------------------
-    const int out_row = a.num_q_heads * a.queries;          // rows of a sequence
-    for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
-        if (paged_len(a, b) > 0) continue;
-        const long long base = (long long)b * out_row * D;
-        for (int i = tid; i < out_row * D; i += kPagedThreads) {
-            if (F32) reinterpret_cast<float*>(a.output)[base + i] = 0.f;
-            else reinterpret_cast<__half*>(a.output)[base + i] = __float2half(0.f);
-        }
-        if (a.lse) for (int i = tid; i < out_row; i += kPagedThreads) a.lse[(long long)b * out_row + i] = -INFINITY;
-    }
-    if (worker >= workers || total == 0) return;
-
-    const long long lo = (long long)worker * total / workers, hi = (long long)(worker + 1) * total / workers;
+    if (lo < hi) {
     PagedCursor at;                                         // what this warp computes
-    at.b = s_start_b[group];
     at.left = hi - lo;
     {
-        const long long rest = s_start_rest[group];
-        const int units = (paged_len(a, at.b) + U - 1) / U;
-        at.hr = (int)(rest / units);
-        at.first = (int)(rest % units);
+        at.b = a.batch > 1 ? s_start_b[group] : 0;
+        cursor_enter<U>(a, at);
+        const int rest = a.batch > 1 ? s_start_rest[group] : lo, hr = rest / at.units;
+        at.first = rest - hr * at.units;
+        at.head = a.row_blocks == 1 ? hr : hr / a.row_blocks;
+        at.rb = a.row_blocks == 1 ? 0 : hr - at.head * a.row_blocks;
+        at.end = min(at.units, at.first + at.left);
     }
-    if (at.left <= 0) return;
-    cursor_enter<U>(a, at);
-    PagedCursor ahead = at;                                 // the unit whose table entries are asked for
-    ahead.u = ahead.first + wi;
+    // ---- the ring: tables, scales, K and V on their way ----------------------------------------------
+    PagedCursor ahead = at;                                 // the unit whose table entries are asked for next
     bool more = true;
-    while (more && ahead.u >= ahead.end) { more = cursor_next_segment<U>(a, ahead); ahead.u = ahead.first + wi; }
-
-    // ---- the ring -----------------------------------------------------------------------------------
-    struct Pending { int page, y, need, head; bool ok; } cur, nxt;
-    cur.page = cur.y = cur.need = cur.head = 0; cur.ok = false;
-    auto look_up = [&]() {                                  // table entries of `ahead`, one box a lane
-        nxt.ok = more;
-        if (!more) return;
-        const int pos = ahead.u * U + (lane << a.box_log2);
-        nxt.need = min(boxes, (ahead.len - ahead.u * U + box_rows - 1) >> a.box_log2);
-        nxt.head = ahead.hr / a.row_blocks;
-        nxt.y = pos & ((1 << a.page_log2) - 1);
-        nxt.page = lane < nxt.need ? __ldg(a.block_table + (long long)ahead.b * a.max_pages + (pos >> a.page_log2)) : 0;
-        ahead.u += gw;
-        while (more && ahead.u >= ahead.end) { more = cursor_next_segment<U>(a, ahead); ahead.u = ahead.first + wi; }
-    };
-    int item = 0, fill_slot = 0;                            // next item to ask for: K of a unit, V of it, K of the next ...
-    auto fill = [&]() {
-        const bool is_v = item & 1;
-        ++item;
-        if (!is_v) { cur = nxt; look_up(); }
-        if (!cur.ok) return;
-        const uint32_t bar = bars_u + fill_slot * 8, dst = ring_u + fill_slot * S::SLOT;
-        int page = cur.page;
-        const bool bad = (unsigned)page >= (unsigned)a.num_pages;
-        if (bad) page = 0;
-        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(cur.need * box_rows * RB));
-        __syncwarp();
-        if (lane < boxes) {
-            const uint32_t sc = scales_u + (fill_slot * 4 + lane) * 4;
-            if (lane < cur.need) {
-                tma_load_pages(dst + lane * box_rows * RB, is_v ? &a.v_map : &a.k_map, cur.y, cur.head, page, bar);
-                if (bad && a.status) *a.status = kStatusBadPage;
-            }
-            if (kScaled && lane < cur.need && !bad) {
-                const float* src = (is_v ? a.v_scale : a.k_scale) + (long long)page * a.num_kv_heads + cur.head;
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc), "l"(src) : "memory");
-            } else {                                        // a page that is not there makes its sequence's rows NaN
-                scales[fill_slot * 4 + lane] = bad ? NAN : 1.f;
-            }
-            if (kScaled) async_copy_arrive(bar);
-        }
-        if (++fill_slot == NS) fill_slot = 0;
-    };
-    look_up();
+    ahead.u = ahead.first + wi;
+    // Table entries are read for as many units of a segment at once as the lanes hold, a batch ahead of their use.
+    struct Batch { int page = 0, u = 0, n = 0, len = 0, head = 0; } cur, nxt;
+    const int box_lanes = 31 - __clz(boxes);                // log2
+    int fill_slot = 0, taken = 0, filled = 0;
+    auto fill = [&]() {                                     // K and V of the next unit, if there is one
 #pragma unroll 1
-    for (int i = 0; i < NS; ++i) fill();
-
-    int slot = 0;
-    uint32_t phase = 0;
-    bool dead = false;
-    auto wait_slot = [&]() {
-        if (!dead && !mbar_wait_bounded(bars_u + slot * 8, phase, nullptr)) {
-            dead = true;
-            if (a.status) *a.status = kStatusFullTimeout;
+        for (int i = 0; i < 2 && taken == cur.n; ++i) {     // (twice where nothing has been looked up yet)
+            cur = nxt;
+            taken = 0;
+            nxt.n = 0;
+            while (more && ahead.u >= ahead.end) { more = cursor_next_segment<U>(a, ahead); ahead.u = ahead.first + wi; }
+            if (!more) continue;
+            nxt.n = min(32 >> box_lanes, (ahead.end - ahead.u + gw - 1) / gw);
+            nxt.u = ahead.u;
+            nxt.len = ahead.len;
+            nxt.head = ahead.head;
+            const int k = lane >> box_lanes;
+            const int pos = (ahead.u + k * gw) * U + ((lane & (boxes - 1)) << a.box_log2);
+            nxt.page = k < nxt.n && pos < ahead.len ? __ldg(a.block_table + (long long)ahead.b * a.max_pages + (pos >> a.page_log2)) : 0;
+            ahead.u += nxt.n * gw;
         }
-        __syncwarp();
-    };
-    auto release_slot = [&]() {                             // read by every lane; filled anew
-        if (++slot == NS) { slot = 0; phase ^= 1; }
-        __syncwarp();
-        if (!dead) fill();
+        if (taken < cur.n) {
+            const int pos = (cur.u + taken * gw) * U, from = taken << box_lanes;
+            const int need = min(boxes, (cur.len - pos + box_rows - 1) >> a.box_log2);
+            const uint32_t bar = bars_u + fill_slot * 8;
+            uint32_t dst = ring_u + fill_slot * S::SLOT;
+            if (elect_one()) mbar_arrive_expect_tx(bar, (uint32_t)(2 * need * box_rows * RB));
+#pragma unroll 1
+            for (int i = 0; i < need; ++i, dst += box_rows * RB) {
+                const int found = __shfl_sync(~0u, cur.page, from + i);
+                const bool bad = (unsigned)found >= (unsigned)a.num_pages;
+                const int page = bad ? 0 : found, y = (pos + (i << a.box_log2)) & ((1 << a.page_log2) - 1);
+                if (elect_one()) {
+                    tma_load_pages(dst, &a.k_map, y, cur.head, page, bar);
+                    tma_load_pages(dst + U * RB, &a.v_map, y, cur.head, page, bar);
+                    const int sc = (filled & 3) * 4 + i;
+                    if (bad) {                              // a page that is not there makes its sequence's rows NaN
+                        scales[sc] = make_float2(NAN, NAN);
+                        if (a.status) *a.status = kStatusBadPage;
+                    } else if (kScaled) {
+                        const long long at_ = (long long)page * a.num_kv_heads + cur.head;
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scales_u + sc * 8), "l"(a.k_scale + at_) : "memory");
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(scales_u + sc * 8 + 4), "l"(a.v_scale + at_) : "memory");
+                    } else scales[sc] = make_float2(1.f, 1.f);
+                }
+            }
+            ++taken;
+            if (++fill_slot == NS) fill_slot = 0;
+        }
+        ++filled;
+        if (kScaled) asm volatile("cp.async.commit_group;" ::: "memory");       // one a call: the scales of a unit are here when NS - 1 are not
     };
 
     const int g4 = lane >> 2, t4 = lane & 3;
-    const int mrow = (lane & 7) + ((lane >> 3) & 1) * 8;    // ldmatrix row and chunk of this lane: K, and V of 8-bit pages
-    const int mchunk = lane >> 4;
-    const int vrow = (lane & 7) + (lane >> 4) * 8;          // V of 16-bit pages
-    const int vchunk = (lane >> 3) & 1;
+    // Where this lane's row of an ldmatrix begins in a slab, for the first two chunks; the chunks of step 2 i are those xor 2 i
+    // (a slab's first row is a multiple of 16, so the swizzle is the same for all slabs).
+    const int block = box_rows * CB;                        // bytes of a column block of a box
+    const uint32_t k_at = box_offset<CB>((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4, 0);                    // K, and V of 8-bit pages
+    const uint32_t v_at = kScaled ? k_at : box_offset<CB>((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1, 0);   // V of 16-bit pages
+    auto chunk_at = [&](uint32_t first, int chunk) { return (first ^ ((chunk % (CB / 16)) * 16)) + (chunk / (CB / 16)) * block; };
+    const int rows_all = a.queries * a.group;
+    const int gt = wi * 32 + lane, gthreads = gw * 32;      // thread of the worker
+    const float2* ml = ml_all + group * gw * ROWS;
 
-    // ---- segments -------------------------------------------------------------------------------------
-    for (;;) {
-        const int head = at.hr / a.row_blocks, rb = at.hr - head * a.row_blocks;
-        const int rows_all = a.queries * a.group;
-        // Q of row n (this lane: n = g4) as B operand
-        uint32_t qf[NT][KSTEPS][2];
-        int limit[NT][2];                                   // positions that the rows of this lane's columns see
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int r = rb * ROWS + nt * 8 + g4;
-            const int j = r / a.group, g = r - j * a.group;
-            const __half* src = a.q + (((long long)at.b * a.queries + j) * a.num_q_heads + head * a.group + g) * D;
-#pragma unroll
-            for (int ks = 0; ks < KSTEPS; ++ks) {
-                if (r < rows_all) {
-                    if (kScaled) {
-                        const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + ks * 16 + t4 * 4));
-                        qf[nt][ks][0] = x.x; qf[nt][ks][1] = x.y;
-                    } else {
-                        qf[nt][ks][0] = __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + t4 * 2));
-                        qf[nt][ks][1] = __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + t4 * 2));
-                    }
-                } else qf[nt][ks][0] = qf[nt][ks][1] = 0;
-            }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int rr = rb * ROWS + nt * 8 + t4 * 2 + e;
-                limit[nt][e] = rr < rows_all ? at.len - a.queries + 1 + rr / a.group : 0;
-            }
-        }
-        float m[NT][2], l[NT][2], o[NT][KSTEPS][4], vref = 0.f;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            m[nt][0] = m[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-            for (int j = 0; j < KSTEPS; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
-        }
-        const int whole = at.len - a.queries + 1;           // positions that every row sees
+    uint32_t qf[NT][KSTEPS][2];                             // Q of row n (this lane: n = g4) as B operand
+    float m[NT][2], l[NT][2], o[NT][KSTEPS][4], vref = 0.f, vmax = 0.f;
+    int slot = 0, u = 0;
+    uint32_t phase = 0;
+    bool fresh = true, dead = false;
 
+    // One turn: a unit computed (none while the ring is filled at first, or where the segment has none for this warp), the
+    // segment closed where it ends, and a unit asked for into the slot that has come free.  One copy of each in the code, which
+    // a short launch spends as much time on fetching as on running.
 #pragma unroll 1
-        for (int u = at.first + wi; u < at.end; u += gw) {
-            const bool ragged = (u + 1) * U > whole;
-            // scores
-            float s[SLABS][NT][4];
+    for (;;) {
+        if (fresh) {
+            fresh = false;
+            u = at.first + wi;
+            vref = vmax = 0.f;
 #pragma unroll
-            for (int sl = 0; sl < SLABS; ++sl)
+            for (int nt = 0; nt < NT; ++nt) {
+                m[nt][0] = m[nt][1] = -INFINITY;
+                l[nt][0] = l[nt][1] = 0.f;
+                const int r = at.rb * ROWS + nt * 8 + g4;
+                const int j = __umulhi(2 * r, a.group_inv), g = r - j * a.group;
+                const __half* src = a.q + (((long long)at.b * a.queries + j) * a.num_q_heads + at.head * a.group + g) * D;
+#pragma unroll
+                for (int ks = 0; ks < KSTEPS; ++ks) {
+                    o[nt][ks][0] = o[nt][ks][1] = o[nt][ks][2] = o[nt][ks][3] = 0.f;
+                    qf[nt][ks][0] = qf[nt][ks][1] = 0;
+                    if (r < rows_all) {
+                        if (kScaled) {
+                            const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + ks * 16 + t4 * 4));
+                            qf[nt][ks][0] = x.x; qf[nt][ks][1] = x.y;
+                        } else {
+                            qf[nt][ks][0] = __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + t4 * 2));
+                            qf[nt][ks][1] = __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + t4 * 2));
+                        }
+                    }
+                }
+            }
+        }
+        bool room = filled < NS;
+        const bool turn = !room;
+        if (turn && u < at.end) {
+            room = true;
+            const int whole = at.len - a.queries + 1;       // positions that every row sees
+            const bool ragged = (u + 1) * U > whole;
+            int limit[NT][2];                               // positions that the rows of this lane's columns see
+            if (ragged) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int r = at.rb * ROWS + nt * 8 + t4 * 2 + e;
+                        limit[nt][e] = r < rows_all ? whole + (int)__umulhi(2 * r, a.group_inv) : 0;
+                    }
+            }
+            if (kScaled) asm volatile("cp.async.wait_group %0;" ::"n"(NS - 1) : "memory");
+            if (!dead && !mbar_wait_bounded(bars_u + slot * 8, phase, nullptr)) {
+                dead = true;
+                if (a.status) *a.status = kStatusFullTimeout;
+            }
+            __syncwarp();
+
+            // ---- scores
+            const uint32_t kbase = ring_u + slot * S::SLOT, vbase = kbase + U * RB;
+            const float2* sc = scales + ((filled - NS) & 3) * 4;
+            float s[SLABS][NT][4], vs[SLABS];
+#pragma unroll
+            for (int sl = 0; sl < SLABS; ++sl) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) s[sl][nt][0] = s[sl][nt][1] = s[sl][nt][2] = s[sl][nt][3] = 0.f;
-            wait_slot();
-            {
-                const uint32_t base = ring_u + slot * S::SLOT;
-                uint32_t slab_at[SLABS];
-                int slab_r[SLABS];
-                float ks_[SLABS];
-#pragma unroll
-                for (int sl = 0; sl < SLABS; ++sl) {
-                    const int box = (sl * 16) >> a.box_log2;
-                    slab_at[sl] = base + box * box_rows * RB;
-                    slab_r[sl] = ((sl * 16) & (box_rows - 1)) + mrow;
-                    ks_[sl] = scales[slot * 4 + box] * a.scale_log2e;
-                }
+                const int box = (sl * 16) >> a.box_log2;
+                const uint32_t from = kbase + box * box_rows * RB + ((sl * 16) & (box_rows - 1)) * CB;
+                const float2 x = sc[box];
+                const float ks_ = x.x * a.scale_log2e;
+                vs[sl] = x.y;
                 if constexpr (kScaled) {
 #pragma unroll
-                    for (int ks = 0; ks < KSTEPS; ks += 2)
+                    for (int ks = 0; ks < KSTEPS; ks += 2) {
+                        uint32_t r0, r1, r2, r3, f0, f1, f2, f3;
+                        ldmatrix_x4(from + chunk_at(k_at, ks), r0, r1, r2, r3);
+                        widen<KIND, false>(r0, f0, f2);
+                        widen<KIND, false>(r1, f1, f3);
 #pragma unroll
-                        for (int sl = 0; sl < SLABS; ++sl) {
-                            uint32_t r0, r1, r2, r3, f0, f1, f2, f3;
-                            ldmatrix_x4(slab_at[sl] + box_offset<CB>(slab_r[sl], ks + mchunk, box_rows), r0, r1, r2, r3);
-                            widen<KIND, false>(r0, f0, f2);
-                            widen<KIND, false>(r1, f1, f3);
+                        for (int nt = 0; nt < NT; ++nt) mma_16816(s[sl][nt], f0, f1, f2, f3, qf[nt][ks][0], qf[nt][ks][1]);
+                        widen<KIND, false>(r2, f0, f2);
+                        widen<KIND, false>(r3, f1, f3);
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_16816(s[sl][nt], f0, f1, f2, f3, qf[nt][ks][0], qf[nt][ks][1]);
-                            widen<KIND, false>(r2, f0, f2);
-                            widen<KIND, false>(r3, f1, f3);
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_16816(s[sl][nt], f0, f1, f2, f3, qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
-                        }
+                        for (int nt = 0; nt < NT; ++nt) mma_16816(s[sl][nt], f0, f1, f2, f3, qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
+                    }
                 } else {
 #pragma unroll
-                    for (int ks = 0; ks < KSTEPS; ++ks)
+                    for (int ks = 0; ks < KSTEPS; ++ks) {
+                        uint32_t f0, f1, f2, f3;
+                        ldmatrix_x4(from + chunk_at(k_at, ks * 2), f0, f1, f2, f3);
 #pragma unroll
-                        for (int sl = 0; sl < SLABS; ++sl) {
-                            uint32_t f0, f1, f2, f3;
-                            ldmatrix_x4(slab_at[sl] + box_offset<CB>(slab_r[sl], ks * 2 + mchunk, box_rows), f0, f1, f2, f3);
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_16816(s[sl][nt], f0, f1, f2, f3, qf[nt][ks][0], qf[nt][ks][1]);
-                        }
+                        for (int nt = 0; nt < NT; ++nt) mma_16816(s[sl][nt], f0, f1, f2, f3, qf[nt][ks][0], qf[nt][ks][1]);
+                    }
                 }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[sl][nt][e] *= ks_;
+            }
+            if (ragged) {
 #pragma unroll
                 for (int sl = 0; sl < SLABS; ++sl)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s[sl][nt][e] *= ks_[sl];
-                            if (ragged && u * U + sl * 16 + g4 + (e >> 1) * 8 >= limit[nt][e & 1]) s[sl][nt][e] = -INFINITY;
-                        }
+                        for (int e = 0; e < 4; ++e)
+                            if (u * U + sl * 16 + g4 + (e >> 1) * 8 >= limit[nt][e & 1]) s[sl][nt][e] = -INFINITY;
             }
-            release_slot();
 
-            // running maximum and sum
+            // ---- running maximum and sum
             float alpha[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -491,34 +495,43 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attention_kernel(const
                     l[nt][e] = l[nt][e] * alpha[nt][e] + sum;
                 }
 
-            wait_slot();
-            {
-                const uint32_t base = ring_u + slot * S::SLOT;
-                if constexpr (kScaled) {
-                    // weights relative to the largest scale so far
-                    float vs[SLABS], top = vref;
+            // O is held in units of `vref`.  A unit of one page makes its scale the unit, which costs nothing beside the
+            // rescaling that O has to have; scales that O could overflow under (2^-40 of the largest), that are zero, not
+            // finite or of extreme size, and units of several pages have their weights multiplied instead.
+            if constexpr (kScaled) {
+                float shrink;
+                if (boxes == 1 && vs[0] >= vmax * 0x1p-40f && vs[0] > 0x1p-100f && vs[0] < 0x1p100f && vref < 0x1p100f) {
+                    shrink = vref == vs[0] ? 1.f : __fdividef(vref, vs[0]);
+                    vref = vs[0];
+                } else {
+                    float top = vref;
 #pragma unroll
                     for (int sl = 0; sl < SLABS; ++sl) {
-                        const int box = (sl * 16) >> a.box_log2;
-                        const bool there = u * U + sl * 16 < at.len;
-                        vs[sl] = there ? scales[slot * 4 + box] : 0.f;
+                        if (u * U + sl * 16 >= at.len) vs[sl] = 0.f;             // a page behind the last one
                         if (!(fabsf(vs[sl]) < INFINITY)) vs[sl] = NAN;
                         top = fmaxf(top, vs[sl]);
                     }
-                    const float shrink = top > 0.f ? vref / top : 1.f;
-                    const float inv = top > 0.f ? 1.f / top : 0.f;
-                    vref = top;
+                    // (steps of 2^64 keep the reciprocal in the normal range)
+                    const float step = top > 1.f ? 0x1p-64f : 0x1p64f, inv = top > 0.f ? __fdividef(1.f, top * step) : 0.f;
+                    shrink = top > 0.f ? vref * step * inv : 1.f;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        alpha[nt][0] *= shrink;
-                        alpha[nt][1] *= shrink;
+                    for (int sl = 0; sl < SLABS; ++sl) {
+                        const float c = vs[sl] * step * inv;
 #pragma unroll
-                        for (int sl = 0; sl < SLABS; ++sl)
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                s[sl][nt][e] = (ragged && s[sl][nt][e] == 0.f) ? 0.f : s[sl][nt][e] * (vs[sl] * inv);
+                            for (int e = 0; e < 4; ++e) s[sl][nt][e] = ragged && s[sl][nt][e] == 0.f ? 0.f : s[sl][nt][e] * c;
                     }
+                    vref = top;
                 }
+                vmax = fmaxf(vmax, vref);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) { alpha[nt][0] *= shrink; alpha[nt][1] *= shrink; }
+            }
+            bool same = true;                               // the maxima and the unit of O are mostly what they were
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) same = same && alpha[nt][0] == 1.f && alpha[nt][1] == 1.f;
+            if (!__all_sync(~0u, same)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -526,90 +539,122 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attention_kernel(const
                         o[nt][j][0] *= alpha[nt][0]; o[nt][j][1] *= alpha[nt][1];
                         o[nt][j][2] *= alpha[nt][0]; o[nt][j][3] *= alpha[nt][1];
                     }
+            }
+
+            // ---- V rows that not every row sees.  They may hold anything, and zero times anything may be NaN: the newest tokens'
+            // rows are added one by one to the rows that see them, and then they and what lies behind them are cleared.
+            if (ragged) {
+                const int from = max(whole - u * U, 0);     // first such position of the unit
+                const int till = min(at.len - u * U, U);
+                if (a.queries > 1 && from < till) {
+                    float* w = reinterpret_cast<float*>(part_all + warp * S::PART) - from * ROWS;
 #pragma unroll
-                for (int sl = 0; sl < SLABS; ++sl) {
-                    uint32_t p[NT][2], pl[NT][2];
+                    for (int sl = 0; sl < SLABS; ++sl)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float x = s[sl][nt][2 * e], y = s[sl][nt][2 * e + 1];
-                            const uint32_t h = pack_half2(x, y);
-                            p[nt][e] = transpose_8x8(h);
-                            if (F32) {
-                                const float2 back = unpack_half2(h);
-                                pl[nt][e] = transpose_8x8(pack_half2(x - back.x, y - back.y));
+                            for (int e = 0; e < 4; ++e) {
+                                const int t = sl * 16 + g4 + (e >> 1) * 8;
+                                if (t >= from && t < till) w[t * ROWS + nt * 8 + t4 * 2 + (e & 1)] = s[sl][nt][e];
+                                if (t >= from) s[sl][nt][e] = 0.f;
                             }
-                        }
-                    const int box = (sl * 16) >> a.box_log2;
-                    const uint32_t at_ = base + box * box_rows * RB;
-                    const int r0_ = (sl * 16) & (box_rows - 1);
-                    // two 16-channel steps of V^T: (f[0..3]) and, of 8-bit pages, (f[4..7])
-                    auto load_v = [&](int j, uint32_t (&f)[8]) {
-                        if constexpr (kScaled) {
-                            uint32_t x0, x1, x2, x3;
-                            ldmatrix_x4_trans(at_ + box_offset<CB>(r0_ + mrow, j + mchunk, box_rows), x0, x1, x2, x3);
-                            widen<KIND, true>(x0, f[0], f[1]);
-                            widen<KIND, true>(x1, f[2], f[3]);
-                            widen<KIND, true>(x2, f[4], f[5]);
-                            widen<KIND, true>(x3, f[6], f[7]);
-                        } else {
-                            ldmatrix_x4_trans(at_ + box_offset<CB>(r0_ + vrow, j * 2 + vchunk, box_rows), f[0], f[1], f[2], f[3]);
-                            ldmatrix_x4_trans(at_ + box_offset<CB>(r0_ + vrow, j * 2 + 2 + vchunk, box_rows), f[4], f[5], f[6], f[7]);
-                        }
-                    };
-                    if (!ragged) {
-#pragma unroll
-                        for (int j = 0; j < KSTEPS; j += 2) {
-                            uint32_t f[8];
-                            load_v(j, f);
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                mma_16816(o[nt][j], f[0], f[1], f[2], f[3], p[nt][0], p[nt][1]);
-                                mma_16816(o[nt][j + 1], f[4], f[5], f[6], f[7], p[nt][0], p[nt][1]);
-                                if (F32) {
-                                    mma_16816(o[nt][j], f[0], f[1], f[2], f[3], pl[nt][0], pl[nt][1]);
-                                    mma_16816(o[nt][j + 1], f[4], f[5], f[6], f[7], pl[nt][0], pl[nt][1]);
-                                }
-                            }
-                        }
-                    } else {
-                        // What a row does not see may be anything: each query token of the block is multiplied with the positions
-                        // behind its limit set to zero, and its own columns are kept.
-                        const int pos = u * U + sl * 16 + t4 * 2;
-                        const int jlo = rb * ROWS / a.group, jhi = min(a.queries - 1, (rb * ROWS + ROWS - 1) / a.group);
+                    __syncwarp();
 #pragma unroll 1
-                        for (int qj = jlo; qj <= jhi; ++qj) {
-                            const int lim = at.len - a.queries + 1 + qj;
-                            if (u * U + sl * 16 >= lim) continue;
-                            const uint32_t k0 = (pos < lim ? 0xffffu : 0u) | (pos + 1 < lim ? 0xffff0000u : 0u);
-                            const uint32_t k1 = (pos + 8 < lim ? 0xffffu : 0u) | (pos + 9 < lim ? 0xffff0000u : 0u);
+                    for (int t = from; t < till; ++t) {
+                        const uint32_t box = vbase + (t >> a.box_log2) * box_rows * RB;
+                        const int row = t & (box_rows - 1);
+                        const float* wt = w + t * ROWS + t4 * 2;
 #pragma unroll
-                            for (int j = 0; j < KSTEPS; j += 2) {
-                                uint32_t f[8];
-                                load_v(j, f);
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                    for (int h = 0; h < 2; ++h) {
-                                        float c[4] = {0.f, 0.f, 0.f, 0.f};
-                                        mma_16816(c, f[4 * h] & k0, f[4 * h + 1] & k0, f[4 * h + 2] & k1, f[4 * h + 3] & k1, p[nt][0], p[nt][1]);
-                                        if (F32) mma_16816(c, f[4 * h] & k0, f[4 * h + 1] & k0, f[4 * h + 2] & k1, f[4 * h + 3] & k1, pl[nt][0], pl[nt][1]);
-                                        if (limit[nt][0] == lim) { o[nt][j + h][0] += c[0]; o[nt][j + h][2] += c[2]; }
-                                        if (limit[nt][1] == lim) { o[nt][j + h][1] += c[1]; o[nt][j + h][3] += c[3]; }
-                                    }
+                        for (int j = 0; j < KSTEPS; ++j) {
+                            float v0, v1;                   // channels of this lane's accumulators
+                            if constexpr (kScaled) {
+                                uint32_t x, y;
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=r"(x) : "r"(box + box_offset<CB>(row, j, block) + g4 * 2));
+                                widen<KIND, false>(x, x, y);
+                                const float2 f = unpack_half2(x);
+                                v0 = f.x; v1 = f.y;
+                            } else {
+                                unsigned short x, y;
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(box + box_offset<CB>(row, j * 2, block) + g4 * 2));
+                                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(y) : "r"(box + box_offset<CB>(row, j * 2 + 1, block) + g4 * 2));
+                                v0 = __half2float(__ushort_as_half(x)); v1 = __half2float(__ushort_as_half(y));
                             }
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    if (u * U + t < limit[nt][e]) {
+                                        o[nt][j][e] += wt[nt * 8 + e] * v0;
+                                        o[nt][j][e + 2] += wt[nt * 8 + e] * v1;
+                                    }
+                        }
+                    }
+                    __syncwarp();
+                }
+#pragma unroll 1
+                for (int i = lane; i < (U - from) * (RB / 16); i += 32) {
+                    const int t = from + i / (RB / 16);
+                    const uint32_t to = vbase + (t >> a.box_log2) * box_rows * RB + box_offset<CB>(t & (box_rows - 1), i % (RB / 16), block);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to), "r"(0) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the slot's next copies come behind these stores
+                __syncwarp();
+            }
+
+            // ---- P V
+#pragma unroll
+            for (int sl = 0; sl < SLABS; ++sl) {
+                uint32_t p[NT][2], pl[NT][2];               // P^T as B operand; its low parts for fp32 output
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float x = s[sl][nt][2 * e], y = s[sl][nt][2 * e + 1];
+                        const uint32_t h = pack_half2(x, y);
+                        p[nt][e] = transpose_8x8(h);
+                        if (F32) {
+                            const float2 back = unpack_half2(h);
+                            pl[nt][e] = transpose_8x8(pack_half2(x - back.x, y - back.y));
+                        }
+                    }
+                const int box = (sl * 16) >> a.box_log2;
+                const uint32_t from = vbase + box * box_rows * RB + ((sl * 16) & (box_rows - 1)) * CB;
+#pragma unroll
+                for (int j = 0; j < KSTEPS; j += 2) {
+                    uint32_t f[8];                          // two 16-channel steps of V^T
+                    if constexpr (kScaled) {
+                        uint32_t x0, x1, x2, x3;
+                        ldmatrix_x4_trans(from + chunk_at(v_at, j), x0, x1, x2, x3);
+                        widen<KIND, true>(x0, f[0], f[1]);
+                        widen<KIND, true>(x1, f[2], f[3]);
+                        widen<KIND, true>(x2, f[4], f[5]);
+                        widen<KIND, true>(x3, f[6], f[7]);
+                    } else {
+                        ldmatrix_x4_trans(from + chunk_at(v_at, j * 2), f[0], f[1], f[2], f[3]);
+                        ldmatrix_x4_trans(from + chunk_at(v_at, j * 2 + 2), f[4], f[5], f[6], f[7]);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_16816(o[nt][j], f[0], f[1], f[2], f[3], p[nt][0], p[nt][1]);
+                        mma_16816(o[nt][j + 1], f[4], f[5], f[6], f[7], p[nt][0], p[nt][1]);
+                        if (F32) {
+                            mma_16816(o[nt][j], f[0], f[1], f[2], f[3], pl[nt][0], pl[nt][1]);
+                            mma_16816(o[nt][j + 1], f[4], f[5], f[6], f[7], pl[nt][0], pl[nt][1]);
                         }
                     }
                 }
             }
-            release_slot();
+            u += gw;
+            if (u >= at.end && lane == 0) s_slot[warp] = slot;
+            if (++slot == NS) { slot = 0; phase ^= 1; }
+            __syncwarp();                                   // the slot has been read by every lane
         }
-
-        // ---- end of the segment: the warps of the worker --------------------------------------------
+        if (turn && u >= at.end) {
+        // ---- end of the segment: the warps of the worker are merged ------------------------------------
         const bool entire = at.first == 0 && at.end == at.units;
-        float gain[NT][2], big[NT][2], sum_l[NT][2];
-        float2* ml = ml_all + warp * ROWS;
+        const bool has_first = at.left == hi - lo;
+        const int rows_here = min(ROWS, rows_all - at.rb * ROWS);
+        const int piece = 2 * worker + (has_first ? 0 : 1);               // where a cut segment's piece goes
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -618,147 +663,146 @@ __global__ void __launch_bounds__(kPagedThreads, 1) paged_attention_kernel(const
                 x += __shfl_xor_sync(~0u, x, 4);
                 x += __shfl_xor_sync(~0u, x, 8);
                 x += __shfl_xor_sync(~0u, x, 16);
-                if (g4 == 0) ml[nt * 8 + t4 * 2 + e] = make_float2(m[nt][e], x);
+                if (g4 == 0) ml_all[warp * ROWS + nt * 8 + t4 * 2 + e] = make_float2(m[nt][e], x);
             }
-        group_barrier(gw, group);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = nt * 8 + t4 * 2 + e;
-                float top = -INFINITY, sum = 0.f;
-                for (int w = 0; w < gw; ++w) top = fmaxf(top, ml_all[(group * gw + w) * ROWS + row].x);
-                const float ref = top == -INFINITY ? 0.f : top;
-                for (int w = 0; w < gw; ++w) {
-                    const float2 x = ml_all[(group * gw + w) * ROWS + row];
-                    sum += x.y * fast_exp2(x.x - ref);
-                }
-                gain[nt][e] = fast_exp2(m[nt][e] - ref) * (kScaled ? vref : 1.f);
-                big[nt][e] = top;
-                sum_l[nt][e] = sum;
-            }
-        // this worker's piece of a cut segment: slot 0 for the one its run begins with, 1 for the one it ends with
-        const bool has_first = at.left == hi - lo;
-        const long long piece = 2ll * worker + (has_first ? 0 : 1);
-        float* my_o = a.part_o + piece * ROWS * D;
-        if (wi == 0 && g4 == 0) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                s_denom[group][nt * 8 + t4 * 2] = sum_l[nt][0];
-                s_denom[group][nt * 8 + t4 * 2 + 1] = sum_l[nt][1];
-            }
-        }
-        if (!entire && wi == 0 && g4 == 0) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    reinterpret_cast<float2*>(a.part_ml)[piece * ROWS + nt * 8 + t4 * 2 + e] = make_float2(big[nt][e], sum_l[nt][e]);
-        }
-        if (entire && a.lse && wi == 0 && g4 == 0) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int r = rb * ROWS + nt * 8 + t4 * 2 + e;
-                    if (r < rows_all) {
-                        const int j = r / a.group;
-                        a.lse[((long long)at.b * a.queries + j) * a.num_q_heads + head * a.group + r - j * a.group] =
-                            sum_l[nt][e] == 0.f ? -INFINITY : (big[nt][e] + log2f(sum_l[nt][e])) * kLn2;
-                    }
-                }
-        }
-        float* buf = merge_all + warp * M::WARP_FLOATS;
-        const float* buf0 = merge_all + group * gw * M::WARP_FLOATS;
-        const int gt = wi * 32 + lane;                      // thread of the worker
-        auto put = [&](int row, int col, float x, float y, float denom) {
-            const int r = rb * ROWS + row;
-            if (r >= rows_all) return;
-            const float inv = denom == 0.f ? 0.f : 1.f / denom;
-            x = denom == 0.f ? 0.f : x * inv;
-            y = denom == 0.f ? 0.f : y * inv;
-            const int j = r / a.group;
-            const long long to = (((long long)at.b * a.queries + j) * a.num_q_heads + head * a.group + r - j * a.group) * D + col;
-            if (F32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.output) + to) = make_float2(x, y);
-            else *reinterpret_cast<__half2*>(reinterpret_cast<__half*>(a.output) + to) = __floats2half2_rn(x, y);
+        auto put = [&](int row, int col, float4 x, float top, float denom) {
+            const int r = at.rb * ROWS + row, j = __umulhi(2 * r, a.group_inv);
+            const long long to = ((long long)at.b * a.queries + j) * a.num_q_heads + at.head * a.group + r - j * a.group;
+            const float inv = __fdividef(1.f, denom);
+            x = denom == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            if (F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.output) + to * D + col) = x;
+            else *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(a.output) + to * D + col) = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
+            if (a.lse && col == 0) a.lse[to] = denom == 0.f ? -INFINITY : (top + __log2f(denom)) * kLn2;
         };
+        // Through the slots that the warps read last.  Columns of rows 2i, 2i + 1 are xored with 8 i: other banks.  A warp that
+        // had no unit of the segment has no such slot, and no weight.
+        const float gain = kScaled ? vref : 1.f;
+        if (at.first + wi < at.end) {
+            float* to = reinterpret_cast<float*>(ring + s_slot[warp] * S::SLOT) + t4 * 2 * D;
 #pragma unroll
-        for (int d0 = 0; d0 < D; d0 += M::DC) {
-            if (d0) group_barrier(gw, group);
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < M::DC / 16; ++j)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const float (&c)[4] = o[nt][d0 / 16 + j];
-                    float* to = buf + (nt * 8 + t4 * 2) * M::LD + j * 16;
+                for (int j = 0; j < KSTEPS; ++j) {
+                    const float (&c)[4] = o[nt][j];
                     if (kScaled) {
-                        *reinterpret_cast<float2*>(to + 2 * g4) = make_float2(c[0] * gain[nt][0], c[2] * gain[nt][0]);
-                        *reinterpret_cast<float2*>(to + M::LD + 2 * g4) = make_float2(c[1] * gain[nt][1], c[3] * gain[nt][1]);
+                        float* at_ = to + nt * 8 * D + ((j * 16 + 2 * g4) ^ (t4 * 8));
+                        *reinterpret_cast<float2*>(at_) = make_float2(c[0] * gain, c[2] * gain);
+                        *reinterpret_cast<float2*>(at_ + D) = make_float2(c[1] * gain, c[3] * gain);
                     } else {
-                        to[g4] = c[0] * gain[nt][0]; to[g4 + 8] = c[2] * gain[nt][0];
-                        to[M::LD + g4] = c[1] * gain[nt][1]; to[M::LD + g4 + 8] = c[3] * gain[nt][1];
+                        float* at_ = to + nt * 8 * D + ((j * 16 + g4) ^ (t4 * 8));
+                        float* at8 = to + nt * 8 * D + ((j * 16 + 8 + g4) ^ (t4 * 8));
+                        at_[0] = c[0]; at8[0] = c[2];
+                        at_[D] = c[1]; at8[D] = c[3];
                     }
                 }
-            group_barrier(gw, group);
-            for (int i = gt; i < ROWS * M::DC / 2; i += gw * 32) {
-                const int row = i / (M::DC / 2), col = i % (M::DC / 2) * 2;
-                float x = 0.f, y = 0.f;
-                for (int w = 0; w < gw; ++w) {
-                    const float2 v = *reinterpret_cast<const float2*>(buf0 + w * M::WARP_FLOATS + row * M::LD + col);
-                    x += v.x; y += v.y;
-                }
-                if (entire) {
-                    put(row, d0 + col, x, y, s_denom[group][row]);
-                } else {
-                    *reinterpret_cast<float2*>(my_o + row * D + d0 + col) = make_float2(x, y);
-                }
+        }
+        group_barrier(gw, group);
+#pragma unroll 1
+        for (int i = gt; i < rows_here * (D / 4); i += gthreads) {
+            const int row = i / (D / 4), col = i % (D / 4) * 4;
+            float top = -INFINITY, denom = 0.f;
+#pragma unroll 4
+            for (int w = 0; w < gw; ++w) top = fmaxf(top, ml[w * ROWS + row].x);
+            const float ref = top == -INFINITY ? 0.f : top;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+            for (int w = 0; w < gw; ++w) {
+                const float2 y = ml[w * ROWS + row];
+                if (y.y == 0.f) continue;
+                const float f = fast_exp2(y.x - ref);
+                const float4 v = *reinterpret_cast<const float4*>(smem + (group * gw + w) * S::RING + s_slot[group * gw + w] * S::SLOT +
+                                                                  (row * D + (col ^ ((row >> 1 & 3) * 8))) * 4);
+                denom += y.y * f;
+                x.x += v.x * f; x.y += v.y * f; x.z += v.z * f; x.w += v.w * f;
+            }
+            if (entire) put(row, col, x, top, denom);
+            else {
+                *reinterpret_cast<float4*>(a.part_o + (piece * ROWS + row) * D + col) = x;
+                if (col == 0) reinterpret_cast<float2*>(a.part_ml)[piece * ROWS + row] = make_float2(top, denom);
             }
         }
         if (!entire) {
             // the workers whose runs hold units of this segment
-            const long long begin = lo + (hi - lo - at.left) - at.first;       // its first unit, of all
-            const long long w0 = ((begin + 1) * workers - 1) / total, w1 = ((begin + at.units) * workers - 1) / total;
-            __threadfence();
+            const int begin = hi - at.left - at.first;      // its first unit, of all
+            const int w0 = begin / per, w1 = (begin + at.units - 1) / per, n = w1 - w0 + 1;
             group_barrier(gw, group);
             if (gt == 0) {
+                __threadfence();                            // for the whole worker: its stores are in front of the barrier
                 const int before = atomicAdd(a.counters + w0, 1);
-                s_last[group] = before == (int)(w1 - w0);
-                if (before == (int)(w1 - w0)) a.counters[w0] = 0;             // ready for the next launch
+                s_last[group] = before == n - 1;
+                if (before == n - 1) a.counters[w0] = 0;    // ready for the next launch
             }
             group_barrier(gw, group);
             if (s_last[group]) {
                 __threadfence();
-                const int n = (int)(w1 - w0) + 1;
-                const long long p0 = 2 * w0 + (w0 * total / workers == begin ? 0 : 1);
-                auto piece_of = [&](int k) { return k == 0 ? p0 : 2 * (w0 + k); };
-                for (int i = gt; i < ROWS * D / 4; i += gw * 32) {
+                const int p0 = 2 * w0 + (w0 * per == begin ? 0 : 1);
+                // `parts` threads take every parts-th piece of four columns of a row, and the first of them joins what they have
+                const int items = rows_here * (D / 4), parts = max(1, min(gthreads / items, 4));
+                float4* join = reinterpret_cast<float4*>(part_all + group * gw * S::PART);
+                float2* join_ml = reinterpret_cast<float2*>(join + gthreads);
+                const int part = parts == 1 ? 0 : gt / items;
+                int i = gt - part * items;
+#pragma unroll 1
+                do {
                     const int row = i / (D / 4), col = i % (D / 4) * 4;
                     float top = -INFINITY, denom = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int k = 0; k < n; ++k) top = fmaxf(top, __ldcg(a.part_ml + (piece_of(k) * ROWS + row) * 2));
-                    const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-                    for (int k = 0; k < n; ++k) {
-                        const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + piece_of(k) * ROWS + row);
-                        const float4 c = __ldcg(reinterpret_cast<const float4*>(a.part_o + (piece_of(k) * ROWS + row) * D + col));
-                        const float f = fast_exp2(v.x - ref);
-                        denom += v.y * f;
-                        x.x += c.x * f; x.y += c.y * f; x.z += c.z * f; x.w += c.w * f;
+                    auto add = [&](float2 y, float4 v) {
+                        const float over = fmaxf(top, y.x), ref = over == -INFINITY ? 0.f : over;
+                        const float old = fast_exp2(top - ref), f = fast_exp2(y.x - ref);
+                        top = over;
+                        denom = denom * old + y.y * f;
+                        x.x = x.x * old + v.x * f; x.y = x.y * old + v.y * f; x.z = x.z * old + v.z * f; x.w = x.w * old + v.w * f;
+                    };
+                    constexpr int AHEAD = 4;
+#pragma unroll 1
+                    for (int k0 = part; k0 < n && i < items && part < parts; k0 += AHEAD * parts) {
+                        float2 y[AHEAD];
+                        float4 v[AHEAD];
+#pragma unroll
+                        for (int q = 0; q < AHEAD; ++q) {
+                            const int k = min(k0 + q * parts, n - 1);
+                            const int from = (k == 0 ? p0 : 2 * (w0 + k)) * ROWS + row;
+                            y[q] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + from);
+                            v[q] = __ldcg(reinterpret_cast<const float4*>(a.part_o + from * D + col));
+                        }
+#pragma unroll
+                        for (int q = 0; q < AHEAD; ++q) if (k0 + q * parts < n) add(y[q], v[q]);
                     }
-                    put(row, col, x.x, x.y, denom);
-                    put(row, col + 2, x.z, x.w, denom);
-                    const int r = rb * ROWS + row;
-                    if (a.lse && col == 0 && r < rows_all) {
-                        const int j = r / a.group;
-                        a.lse[((long long)at.b * a.queries + j) * a.num_q_heads + head * a.group + r - j * a.group] =
-                            denom == 0.f ? -INFINITY : (top + log2f(denom)) * kLn2;
+                    if (parts > 1) {
+                        join[gt] = x;
+                        join_ml[gt] = make_float2(top, denom);
+                        group_barrier(gw, group);
+#pragma unroll 1
+                        for (int q = 1; q < parts && part == 0; ++q) add(join_ml[q * items + gt], join[q * items + gt]);
                     }
-                }
+                    if (i < items && part == 0) put(row, col, x, top, denom);
+                    i += gthreads;
+                } while (parts == 1 && i < items);
             }
         }
-        group_barrier(gw, group);                           // the merge buffers are free again
         if (!cursor_next_segment<U>(a, at)) break;
+        fresh = true;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");             // the slot's next copies come behind these accesses
+        group_barrier(gw, group);                           // what was merged has been read
+        }
+        if (room && !dead) fill();
+    }
+    }
+
+    // ---- rows of sequences without positions; positions that no table holds -------------------------------
+    if (total > 0 && lives == a.batch && a.status == nullptr) return;
+    for (int b = blockIdx.x * W + warp; b < a.batch; b += grid * W) {
+        const int off = __ldg(a.kv_offsets + b);
+        if (lane == 0 && a.status && off >= (a.max_pages << a.page_log2)) *a.status = kStatusBadPosition;
+        if (off >= 0) continue;
+        const int rows = a.num_q_heads * a.queries;
+        const long long first = (long long)b * rows;
+        for (int i = lane; i < rows * (D / 4); i += 32) {
+            if (F32) reinterpret_cast<float4*>(a.output)[first * (D / 4) + i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            else reinterpret_cast<uint2*>(a.output)[first * (D / 4) + i] = make_uint2(0u, 0u);
+        }
+        if (a.lse) for (int i = lane; i < rows; i += 32) a.lse[first + i] = -INFINITY;
     }
 }
 

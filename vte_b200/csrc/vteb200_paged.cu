@@ -45,10 +45,11 @@ int check_cache(const vteb_paged_cache_t* c) {
     return 0;
 }
 
-// Positions of a box of the tensor maps: a page, or as much of it as a unit of the attention kernel holds.
+int row_bytes_of(int head_dim, int type) { return head_dim * (type == kPagedF16 ? 2 : 1); }
+
+// Positions of a box of the tensor maps: as many as a unit of the attention kernel holds.
 int box_rows_of(int head_dim, int type, int page_size) {
-    const int rb = head_dim * (type == kPagedF16 ? 2 : 1);
-    const int unit = rb == 64 ? 64 : rb <= 256 ? 32 : 16;
+    const int unit = paged_unit(row_bytes_of(head_dim, type));
     return page_size < unit ? page_size : unit;
 }
 
@@ -71,9 +72,9 @@ struct Workspace { size_t counters, ml, o, bytes; };
 Workspace workspace_of(int rows, int head_dim, int sms) {
     const int block = rows_per_block(rows, head_dim);
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-    const size_t pieces = 2 * (size_t)sms * kPagedWarps;
+    const size_t pieces = 2 * (size_t)sms * paged_warps(head_dim, head_dim, block / 8);      // (16-bit rows take no more warps)
     Workspace w;
-    w.counters = up((size_t)sms * kPagedWarps * 4);
+    w.counters = up((size_t)sms * 16 * 4);
     w.ml = up(pieces * block * 8);
     w.o = up(pieces * block * (size_t)head_dim * 4);
     w.bytes = w.counters + w.ml + w.o;
@@ -90,20 +91,39 @@ int check_heads(int q_heads, int kv_heads, int head_dim, int batch, int query_to
     return 0;
 }
 
-typedef void (*AttnKernel)(const PagedAttnArgs);
+struct AttnKernel { void (*fn)(const PagedAttnArgs); int threads, smem; };
+
+template <int D, int KIND, int NT>
+AttnKernel attention_of(bool f32) {
+    using S = PagedShape<D, KIND, NT>;
+    return {f32 ? paged_attention_kernel<D, KIND, NT, true> : paged_attention_kernel<D, KIND, NT, false>, S::W * 32, S::SMEM};
+}
 
 template <int D, int KIND>
 AttnKernel attention_of(int block, bool f32) {
-    if constexpr (D < 256) {
-        if (block == 16) return f32 ? paged_attention_kernel<D, KIND, 2, true> : paged_attention_kernel<D, KIND, 2, false>;
-    }
-    return f32 ? paged_attention_kernel<D, KIND, 1, true> : paged_attention_kernel<D, KIND, 1, false>;
+    if constexpr (D < 256) { if (block == 16) return attention_of<D, KIND, 2>(f32); }
+    return attention_of<D, KIND, 1>(f32);
 }
 
 template <int D>
 AttnKernel attention_of(int type, int block, bool f32) {
     return type == kPagedF16 ? attention_of<D, kPagedF16>(block, f32)
          : type == kPagedE4m3 ? attention_of<D, kPagedE4m3>(block, f32) : attention_of<D, kPagedInt8>(block, f32);
+}
+
+template <typename Args>
+int launch(void (*fn)(const Args), const Args& args, unsigned grid, unsigned threads, int smem, void* stream, bool programmatic, const char* what) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    if (programmatic) { cfg.attrs = &attr; cfg.numAttrs = 1; }
+    return report_rt(cudaLaunchKernelEx(&cfg, fn, args), what);
 }
 
 typedef void (*AppendKernel)(const PagedAppendArgs);
@@ -215,8 +235,7 @@ int vteb_paged_append(const vteb_paged_cache_t* c, const vteb_paged_append_t* a,
     if (kv_blocks + q_blocks > INT_MAX) return report(VTEB_ERR_TOO_LARGE, "%d tokens: too many blocks", a->total_tokens);
     p.kv_blocks = (int)kv_blocks;
     AppendKernel k = c->type == kPagedF16 ? append_of<0>(it) : c->type == kPagedE4m3 ? append_of<1>(it) : append_of<2>(it);
-    k<<<dim3((unsigned)(kv_blocks + q_blocks)), dim3(threads), 0, (cudaStream_t)stream>>>(p);
-    return report_rt(cudaGetLastError(), "paged append launch");
+    return launch(k, p, (unsigned)(kv_blocks + q_blocks), threads, 0, stream, (a->launch_flags & VTEB_LAUNCH_PROGRAMMATIC) != 0, "paged append launch");
 }
 
 int vteb_paged_attention_workspace(int num_q_heads, int num_kv_heads, int head_dim, int batch, int query_tokens, size_t* bytes) {
@@ -245,6 +264,9 @@ int vteb_paged_attention(const vteb_paged_cache_t* c, const vteb_paged_attention
     if ((rc = sm_count(&sms))) return rc;
     const int group = a->num_q_heads / c->num_kv_heads, rows = a->query_tokens * group;
     const int block = rows_per_block(rows, c->head_dim);
+    const int unit = paged_unit(row_bytes_of(c->head_dim, c->type)), blocks = (rows + block - 1) / block;
+    if ((long long)a->batch * c->num_kv_heads * blocks * (((long long)a->max_pages * c->page_size + unit - 1) / unit + 16) > INT_MAX / 2)
+        return report(VTEB_ERR_TOO_LARGE, "%d sequences of up to %d pages: more work than a launch counts", a->batch, a->max_pages);
     const Workspace w = workspace_of(rows, c->head_dim, sms);
     if (a->workspace_bytes < w.bytes) return report(VTEB_ERR_TOO_LARGE, "the workspace holds %zu of %zu bytes", a->workspace_bytes, w.bytes);
     PagedAttnArgs p;
@@ -263,20 +285,19 @@ int vteb_paged_attention(const vteb_paged_cache_t* c, const vteb_paged_attention
     p.box_log2 = log2_of(box_rows_of(c->head_dim, c->type, c->page_size));
     p.num_q_heads = a->num_q_heads; p.num_kv_heads = c->num_kv_heads; p.group = group; p.queries = a->query_tokens;
     p.row_blocks = (rows + block - 1) / block;
+    p.group_inv = ((1u << 31) + group - 1) / group;
     p.scale_log2e = a->scale * kLog2e;
     const bool f32 = a->out_is_f32 != 0;
     AttnKernel k = c->head_dim == 64 ? attention_of<64>(c->type, block, f32)
                  : c->head_dim == 128 ? attention_of<128>(c->type, block, f32) : attention_of<256>(c->type, block, f32);
-    const int smem = block == 16 ? paged_smem_bytes<2>() : paged_smem_bytes<1>();
     static bool raised[64][3][3][2][2];
     const int dev = vteb_shim::device_index(), di = log2_of(c->head_dim) - 6;
     const bool known = dev < 64;
     if (!known || !raised[dev][di][c->type][block == 16][f32]) {
-        if ((rc = report_rt(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute(max dynamic shared memory)"))) return rc;
+        if ((rc = report_rt(cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem), "cudaFuncSetAttribute(max dynamic shared memory)"))) return rc;
         if (known) raised[dev][di][c->type][block == 16][f32] = true;
     }
-    k<<<dim3(sms), dim3(kPagedThreads), smem, (cudaStream_t)stream>>>(p);
-    return report_rt(cudaGetLastError(), "paged attention launch");
+    return launch(k.fn, p, sms, k.threads, k.smem, stream, (a->launch_flags & VTEB_LAUNCH_PROGRAMMATIC) != 0, "paged attention launch");
 }
 
 }  // extern "C"
