@@ -8,7 +8,7 @@
 //
 // Work.  The positions of a sequence are cut into units of U positions (4 to 8 KB of K and as much of V); (sequence, KV
 // head, block of rows) is a segment, and all units of all segments, in that order, are dealt as equal runs to the
-// workers.  A worker is `gw` of the warps of a CTA, one CTA an SM: the runs and `gw` are computed on the device from the
+// workers.  A worker is all or half of the `W` warps of a CTA, one CTA an SM: the runs are computed on the device from the
 // step's own lengths.  Each warp of a worker takes every gw-th unit and has a ring of its own in shared memory, which its own
 // lanes fill with tensor-map copies (one box a page) and which only it reads: no warp waits for another between the
 // ends of segments, and the loads of the next segment are in flight while one is merged.
@@ -56,28 +56,28 @@ struct PagedAttnArgs {
 };
 
 // Positions of a unit (4 or 8 KB of K, and as much of V) and warps of a CTA, so that the rings (192 KB of an SM's 227) hold at
-// least two units a warp and a thread's accumulators, Q fragments and scores fit its registers (168 with 12 warps).
+// least two units a warp.  Few warps with many registers: a warp's own loads, conversions and products overlap, which twelve
+// of 168 registers or sixteen of 128 do less well (64 sequences of 8 x 64-wide e4m3 heads 103, 114 and 217 us).
 __host__ __device__ constexpr int paged_unit(int row_bytes) { return row_bytes >= 256 ? 16 : 4096 / row_bytes; }
-__host__ __device__ constexpr int paged_warps(int row_bytes, int head_dim, int nt) {
-    return row_bytes == 512 ? 6 : head_dim * nt == 256 ? 8 : 12;
-}
+__host__ __device__ constexpr int paged_warps(int row_bytes) { return row_bytes == 512 ? 6 : 8; }
+constexpr int kPagedMaxWorkers = 2;      // of a CTA
 
 template <int D, int KIND, int NT>
 struct PagedShape {
     static constexpr int ES = KIND == kPagedF16 ? 2 : 1;
     static constexpr int RB = D * ES;                       // bytes of a row
     static constexpr int CB = RB < 128 ? RB : 128;          // bytes of a column block: the width of a box
-    static constexpr int W = paged_warps(RB, D, NT);
+    static constexpr int W = paged_warps(RB);
     static constexpr int RING = 192 * 1024 / W;             // bytes of a warp's ring
     static constexpr int U = paged_unit(RB);                           // positions of a unit
     static constexpr int SLOT = 2 * U * RB;                 // K, then V
     static constexpr int NS = RING / SLOT;
     static constexpr int ROWS = 8 * NT;
-    static constexpr int PART = 1024;                       // bytes a warp has for the last merge's parts, and for the newest tokens' weights
+    static constexpr int PART = 1024;                       // bytes a warp has for the newest tokens' weights
     static constexpr int SMEM = 1024 + W * (RING + PART + ROWS * 8 + 4 * 4 * 8 + 64);
     static_assert(NS >= 2 && NS <= 4, "units in a ring");
     static_assert(ROWS * D * 4 <= SLOT, "a warp's rows fit the slot that it read last");
-    static_assert(PART >= 32 * 24 && PART >= 15 * ROWS * 4, "parts and weights");
+    static_assert(PART >= 15 * ROWS * 4, "weights of the newest tokens");
 };
 
 #if defined(__CUDACC__)
@@ -136,8 +136,7 @@ __device__ __forceinline__ uint32_t box_offset(int r, int chunk, int block) {
 }
 
 __device__ __forceinline__ void group_barrier(int gw, int group) {
-    if (gw == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(gw * 32) : "memory");
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(gw * 32) : "memory");
 }
 
 // Where a warp is in its worker's run: unit `u` of a segment, of which units [first, end) are this worker's.
@@ -187,7 +186,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
     constexpr bool kScaled = KIND != kPagedF16;
 
     extern __shared__ unsigned char smem_raw[];
-    __shared__ int s_scan[W], s_live[W], s_start_b[W], s_start_rest[W], s_last[W], s_slot[W];
+    __shared__ int s_scan[W], s_live[W], s_start_b[kPagedMaxWorkers], s_start_rest[kPagedMaxWorkers], s_last[kPagedMaxWorkers], s_slot[W];
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -249,16 +248,16 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
         }
     }
     total *= HR;
-    // Workers of a CTA.
+    // Workers of a CTA: two where there are segments for all of them, so that one computes while the other merges (64 sequences
+    // of 8 x 64-wide e4m3 heads: 114 us with one, 103 with two, 104 with four); one where few segments are cut often
+    // (32,768 positions of 2 x 128-wide e4m3 heads: 15 and 19 us).
     const int segments = lives * HR, grid = gridDim.x;
-    int groups = 1;
-    while (groups < W) {                                    // 1, 2, 4, 12 or 1, 2, 4, 8 or 1, 2, 6
-        const int more = W % 8 && groups * 4 > W ? W : groups * 2;
-        if (segments * 4 < grid * more || (total < grid * more * 16 && total >= segments * (W / more) * 2)) break;
-        groups = more;
-    }
-    const int gw = W / groups, group = groups == 1 ? 0 : warp / gw, wi = groups == 1 ? warp : warp - group * gw;
-    const int per = max((total + grid * groups - 1) / (grid * groups), gw);              // units of a worker
+    const int groups = segments >= grid ? kPagedMaxWorkers : 1;
+    const int gw = W / groups, group = groups == 1 ? 0 : warp / (W / 2), wi = groups == 1 ? warp : warp % (W / 2);
+    // Units of a worker: an equal share, but not so few that a segment is cut where its warps would have little to do each.
+    constexpr int kUnitsOfAWarp = 2;
+    const int mean = segments ? (total + segments - 1) / segments : 1, cuts = (mean + kUnitsOfAWarp * gw - 1) / (kUnitsOfAWarp * gw);
+    const int per = max((total + grid * groups - 1) / (grid * groups), (mean + cuts - 1) / cuts);
     const int worker = blockIdx.x * groups + group;
     const int lo = worker * per, hi = min(lo + per, total);
     if (a.batch > 1) {
@@ -360,6 +359,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
 
     uint32_t qf[NT][KSTEPS][2];                             // Q of row n (this lane: n = g4) as B operand
     float m[NT][2], l[NT][2], o[NT][KSTEPS][4], vref = 0.f, vmax = 0.f;
+    if (lane == 0) s_slot[warp] = 0;                        // a warp that computes nothing is read, and not used
     int slot = 0, u = 0;
     uint32_t phase = 0;
     bool fresh = true, dead = false;
@@ -665,13 +665,13 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                 x += __shfl_xor_sync(~0u, x, 16);
                 if (g4 == 0) ml_all[warp * ROWS + nt * 8 + t4 * 2 + e] = make_float2(m[nt][e], x);
             }
-        auto put = [&](int row, int col, float4 x, float top, float denom) {
+        auto put = [&](int row, int col, float2 x, float top, float denom) {
             const int r = at.rb * ROWS + row, j = __umulhi(2 * r, a.group_inv);
             const long long to = ((long long)at.b * a.queries + j) * a.num_q_heads + at.head * a.group + r - j * a.group;
             const float inv = __fdividef(1.f, denom);
-            x = denom == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-            if (F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.output) + to * D + col) = x;
-            else *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(a.output) + to * D + col) = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
+            x = denom == 0.f ? make_float2(0.f, 0.f) : make_float2(x.x * inv, x.y * inv);
+            if (F32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.output) + to * D + col) = x;
+            else *reinterpret_cast<uint32_t*>(reinterpret_cast<__half*>(a.output) + to * D + col) = pack_half2(x.x, x.y);
             if (a.lse && col == 0) a.lse[to] = denom == 0.f ? -INFINITY : (top + __log2f(denom)) * kLn2;
         };
         // Through the slots that the warps read last.  Columns of rows 2i, 2i + 1 are xored with 8 i: other banks.  A warp that
@@ -698,26 +698,38 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
         }
         group_barrier(gw, group);
 #pragma unroll 1
-        for (int i = gt; i < rows_here * (D / 4); i += gthreads) {
-            const int row = i / (D / 4), col = i % (D / 4) * 4;
+        for (int i = gt; i < rows_here * (D / 2); i += gthreads) {
+            const int row = i / (D / 2), col = i % (D / 2) * 2;
             float top = -INFINITY, denom = 0.f;
-#pragma unroll 4
-            for (int w = 0; w < gw; ++w) top = fmaxf(top, ml[w * ROWS + row].x);
-            const float ref = top == -INFINITY ? 0.f : top;
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-            for (int w = 0; w < gw; ++w) {
-                const float2 y = ml[w * ROWS + row];
-                if (y.y == 0.f) continue;
-                const float f = fast_exp2(y.x - ref);
-                const float4 v = *reinterpret_cast<const float4*>(smem + (group * gw + w) * S::RING + s_slot[group * gw + w] * S::SLOT +
-                                                                  (row * D + (col ^ ((row >> 1 & 3) * 8))) * 4);
-                denom += y.y * f;
-                x.x += v.x * f; x.y += v.y * f; x.z += v.z * f; x.w += v.w * f;
+            float2 x = make_float2(0.f, 0.f);
+#pragma unroll 1
+            for (int w0 = 0; w0 < gw; w0 += 4) {            // four warps at a time, so that their reads are under way together
+                float2 y[4];
+                float2 v[4];
+                float over = top;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int w = min(w0 + q, gw - 1);
+                    y[q] = ml[w * ROWS + row];
+                    v[q] = *reinterpret_cast<const float2*>(smem + (group * gw + w) * S::RING + s_slot[group * gw + w] * S::SLOT +
+                                                            (row * D + (col ^ ((row >> 1 & 3) * 8))) * 4);
+                    if (w0 + q >= gw) y[q] = make_float2(-INFINITY, 0.f);
+                    over = fmaxf(over, y[q].x);
+                }
+                const float ref = over == -INFINITY ? 0.f : over, old = fast_exp2(top - ref);
+                top = over;
+                denom *= old;
+                x.x *= old; x.y *= old;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float f = fast_exp2(y[q].x - ref);
+                    denom += y[q].y * f;
+                    if (y[q].y != 0.f) { x.x += v[q].x * f; x.y += v[q].y * f; }
+                }
             }
             if (entire) put(row, col, x, top, denom);
             else {
-                *reinterpret_cast<float4*>(a.part_o + (piece * ROWS + row) * D + col) = x;
+                *reinterpret_cast<float2*>(a.part_o + (piece * ROWS + row) * D + col) = x;
                 if (col == 0) reinterpret_cast<float2*>(a.part_ml)[piece * ROWS + row] = make_float2(top, denom);
             }
         }
@@ -736,49 +748,40 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             if (s_last[group]) {
                 __threadfence();
                 const int p0 = 2 * w0 + (w0 * per == begin ? 0 : 1);
-                // `parts` threads take every parts-th piece of four columns of a row, and the first of them joins what they have
-                const int items = rows_here * (D / 4), parts = max(1, min(gthreads / items, 4));
-                float4* join = reinterpret_cast<float4*>(part_all + group * gw * S::PART);
-                float2* join_ml = reinterpret_cast<float2*>(join + gthreads);
-                const int part = parts == 1 ? 0 : gt / items;
-                int i = gt - part * items;
+                // Four columns a thread, the pieces in order: many reads on their way, as they come from L2.
 #pragma unroll 1
-                do {
+                for (int i = gt; i < rows_here * (D / 4); i += gthreads) {
                     const int row = i / (D / 4), col = i % (D / 4) * 4;
                     float top = -INFINITY, denom = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    auto add = [&](float2 y, float4 v) {
-                        const float over = fmaxf(top, y.x), ref = over == -INFINITY ? 0.f : over;
-                        const float old = fast_exp2(top - ref), f = fast_exp2(y.x - ref);
-                        top = over;
-                        denom = denom * old + y.y * f;
-                        x.x = x.x * old + v.x * f; x.y = x.y * old + v.y * f; x.z = x.z * old + v.z * f; x.w = x.w * old + v.w * f;
-                    };
-                    constexpr int AHEAD = 4;
+                    constexpr int AHEAD = 16;
 #pragma unroll 1
-                    for (int k0 = part; k0 < n && i < items && part < parts; k0 += AHEAD * parts) {
+                    for (int k0 = 0; k0 < n; k0 += AHEAD) {
                         float2 y[AHEAD];
                         float4 v[AHEAD];
 #pragma unroll
                         for (int q = 0; q < AHEAD; ++q) {
-                            const int k = min(k0 + q * parts, n - 1);
-                            const int from = (k == 0 ? p0 : 2 * (w0 + k)) * ROWS + row;
+                            const int k = min(k0 + q, n - 1), from = (k == 0 ? p0 : 2 * (w0 + k)) * ROWS + row;
                             y[q] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + from);
                             v[q] = __ldcg(reinterpret_cast<const float4*>(a.part_o + from * D + col));
                         }
+                        float over = top;
 #pragma unroll
-                        for (int q = 0; q < AHEAD; ++q) if (k0 + q * parts < n) add(y[q], v[q]);
+                        for (int q = 0; q < AHEAD; ++q) over = fmaxf(over, y[q].x);      // (one that is read twice does no harm here)
+                        const float ref = over == -INFINITY ? 0.f : over, old = fast_exp2(top - ref);
+                        top = over;
+                        denom *= old;
+                        x.x *= old; x.y *= old; x.z *= old; x.w *= old;
+#pragma unroll
+                        for (int q = 0; q < AHEAD; ++q) {
+                            const float f = k0 + q < n ? fast_exp2(y[q].x - ref) : 0.f;
+                            denom += y[q].y * f;
+                            x.x += v[q].x * f; x.y += v[q].y * f; x.z += v[q].z * f; x.w += v[q].w * f;
+                        }
                     }
-                    if (parts > 1) {
-                        join[gt] = x;
-                        join_ml[gt] = make_float2(top, denom);
-                        group_barrier(gw, group);
-#pragma unroll 1
-                        for (int q = 1; q < parts && part == 0; ++q) add(join_ml[q * items + gt], join[q * items + gt]);
-                    }
-                    if (i < items && part == 0) put(row, col, x, top, denom);
-                    i += gthreads;
-                } while (parts == 1 && i < items);
+                    put(row, col, make_float2(x.x, x.y), top, denom);
+                    put(row, col + 2, make_float2(x.z, x.w), top, denom);
+                }
             }
         }
         if (!cursor_next_segment<U>(a, at)) break;

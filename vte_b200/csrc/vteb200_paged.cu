@@ -72,9 +72,9 @@ struct Workspace { size_t counters, ml, o, bytes; };
 Workspace workspace_of(int rows, int head_dim, int sms) {
     const int block = rows_per_block(rows, head_dim);
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-    const size_t pieces = 2 * (size_t)sms * paged_warps(head_dim, head_dim, block / 8);      // (16-bit rows take no more warps)
+    const size_t workers = (size_t)sms * kPagedMaxWorkers, pieces = 2 * workers;
     Workspace w;
-    w.counters = up((size_t)sms * 16 * 4);
+    w.counters = up(workers * 4);
     w.ml = up(pieces * block * 8);
     w.o = up(pieces * block * (size_t)head_dim * 4);
     w.bytes = w.counters + w.ml + w.o;
