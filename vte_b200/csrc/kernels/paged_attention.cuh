@@ -61,6 +61,8 @@ struct PagedAttnArgs {
 __host__ __device__ constexpr int paged_unit(int row_bytes) { return row_bytes >= 256 ? 16 : 4096 / row_bytes; }
 __host__ __device__ constexpr int paged_warps(int row_bytes) { return row_bytes == 512 ? 6 : 8; }
 constexpr int kPagedMaxWorkers = 2;      // of a CTA
+// Measured in paged_attention_kernel, where they are used.
+constexpr int kPagedTwoFrom = 4, kPagedAligned = 8, kPagedUnitsOfAWarp = 2;
 
 template <int D, int KIND, int NT>
 struct PagedShape {
@@ -215,58 +217,72 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
     const int HR = a.num_kv_heads * a.row_blocks;
 
     // ---- all units, and where this CTA's workers begin ------------------------------------------
-    int total, lives, mine = 0, upto = 0, b0 = 0, b1 = 1;
-    if (a.batch == 1) {
-        total = (paged_len(a, 0) + U - 1) / U;
-        lives = total > 0;
-        __syncwarp();
-    } else {
-        const int per_thread = (a.batch + W * 32 - 1) / (W * 32);
-        b0 = min(tid * per_thread, a.batch);
-        b1 = min(b0 + per_thread, a.batch);
-        int live = 0;
-        for (int b = b0; b < b1; ++b) {
-            const int units = (paged_len(a, b) + U - 1) / U;
-            mine += units;
-            live += units > 0;
-        }
+    auto units_of = [&](int b) { return (paged_len(a, b) + U - 1) / U; };
+    const int per_thread = (a.batch + W * 32 - 1) / (W * 32);
+    const int b0 = min(tid * per_thread, a.batch), b1 = min(b0 + per_thread, a.batch);
+    int total = 0, lives = 0, mine = 0, upto = 0;
+    auto scan = [&](auto units) {                           // this thread's sequences, all up to them, all
+        mine = 0;
+        for (int b = b0; b < b1; ++b) mine += units(b);
         upto = mine;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int x = __shfl_up_sync(~0u, upto, d);
             if (lane >= d) upto += x;
         }
-        live = __reduce_add_sync(~0u, live);
-        if (lane == 31) { s_scan[warp] = upto; s_live[warp] = live; }
+        if (lane == 31) s_scan[warp] = upto;
         __syncthreads();
-        total = lives = 0;
+        total = 0;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
             if (w < warp) upto += s_scan[w];
             total += s_scan[w];
-            lives += s_live[w];
         }
+    };
+    if (a.batch == 1) {
+        total = units_of(0);
+        lives = total > 0;
+        __syncwarp();
+    } else {
+        int live = 0;
+        for (int b = b0; b < b1; ++b) live += units_of(b) > 0;
+        live = __reduce_add_sync(~0u, live);
+        if (lane == 0) s_live[warp] = live;
+        scan(units_of);
+#pragma unroll
+        for (int w = 0; w < W; ++w) lives += s_live[w];
     }
     total *= HR;
-    // Workers of a CTA: two where there are segments for all of them, so that one computes while the other merges (64 sequences
-    // of 8 x 64-wide e4m3 heads: 114 us with one, 103 with two, 104 with four); one where few segments are cut often
-    // (32,768 positions of 2 x 128-wide e4m3 heads: 15 and 19 us).
+    // Workers of a CTA: two where there are segments for them, so that one computes while the other merges (64 sequences of
+    // 8 x 64-wide e4m3 heads: 114 us with one, 103 with two, 104 with four); one where few segments would be cut more often
+    // for that (32,768 positions of 2 x 128-wide e4m3 heads: 15 and 19 us).
     const int segments = lives * HR, grid = gridDim.x;
-    const int groups = segments >= grid ? kPagedMaxWorkers : 1;
+    const int groups = segments * kPagedTwoFrom >= grid ? kPagedMaxWorkers : 1, workers = grid * groups;
     const int gw = W / groups, group = groups == 1 ? 0 : warp / (W / 2), wi = groups == 1 ? warp : warp % (W / 2);
     // Units of a worker: an equal share, but not so few that a segment is cut where its warps would have little to do each.
-    constexpr int kUnitsOfAWarp = 2;
-    const int mean = segments ? (total + segments - 1) / segments : 1, cuts = (mean + kUnitsOfAWarp * gw - 1) / (kUnitsOfAWarp * gw);
-    const int per = max((total + grid * groups - 1) / (grid * groups), (mean + cuts - 1) / cuts);
+    // Short runs begin with a segment each: `per` units stand for what is left of one, so that no worker has parts of two.
+    const bool aligned = segments * 2 <= workers && total < workers * gw * kPagedAligned;
+    const int mean = segments ? (total + segments - 1) / segments : 1, cuts = (mean + kPagedUnitsOfAWarp * gw - 1) / (kPagedUnitsOfAWarp * gw);
+    const int over = !aligned ? workers : a.batch == 1 ? workers / segments * segments : workers - segments;
+    const int per = max((total + over - 1) / over, (mean + cuts - 1) / cuts);
+    auto room_of = [&](int units) { return aligned ? (units + per - 1) / per * per : units; };
+    if (aligned) {
+        if (a.batch == 1) total = room_of(mean) * segments;
+        else {
+            __syncthreads();                                // s_scan is written anew
+            scan([&](int b) { return room_of(units_of(b)); });
+            total *= HR;
+        }
+    }
     const int worker = blockIdx.x * groups + group;
-    const int lo = worker * per, hi = min(lo + per, total);
+    const int lo = worker * per;
     if (a.batch > 1) {
         for (int g = 0; g < groups; ++g) {
             const int at = (blockIdx.x * groups + g) * per;
             if (at >= (upto - mine) * HR && at < upto * HR) {
                 int rest = at - (upto - mine) * HR, b = b0;
                 for (; b < b1; ++b) {
-                    const int n = (paged_len(a, b) + U - 1) / U * HR;
+                    const int n = room_of(units_of(b)) * HR;
                     if (rest < n) break;
                     rest -= n;
                 }
@@ -277,18 +293,19 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
         __syncthreads();
     }
 
-    if (lo < hi) {
+    if (lo < total) {
     PagedCursor at;                                         // what this warp computes
-    at.left = hi - lo;
     {
         at.b = a.batch > 1 ? s_start_b[group] : 0;
         cursor_enter<U>(a, at);
-        const int rest = a.batch > 1 ? s_start_rest[group] : lo, hr = rest / at.units;
-        at.first = rest - hr * at.units;
+        const int rest = a.batch > 1 ? s_start_rest[group] : lo, room = room_of(at.units), hr = rest / room;
+        at.first = rest - hr * room;
+        at.left = min(per, (aligned ? at.units - at.first : total - lo));
         at.head = a.row_blocks == 1 ? hr : hr / a.row_blocks;
         at.rb = a.row_blocks == 1 ? 0 : hr - at.head * a.row_blocks;
         at.end = min(at.units, at.first + at.left);
     }
+    const int hi = lo + at.left;
     // ---- the ring: tables, scales, K and V on their way ----------------------------------------------
     PagedCursor ahead = at;                                 // the unit whose table entries are asked for next
     bool more = true;
