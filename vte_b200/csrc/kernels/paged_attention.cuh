@@ -765,13 +765,14 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             if (s_last[group]) {
                 __threadfence();
                 const int p0 = 2 * w0 + (w0 * per == begin ? 0 : 1);
-                // Four columns a thread, the pieces in order: many reads on their way, as they come from L2.
+                // Four columns a thread, the pieces in order: eight reads of each on their way, as they come from L2 (sixteen take registers that the
+                // main loop needs: 16 ragged int8 sequences of 256-wide heads 90 and 95 us).
 #pragma unroll 1
                 for (int i = gt; i < rows_here * (D / 4); i += gthreads) {
                     const int row = i / (D / 4), col = i % (D / 4) * 4;
                     float top = -INFINITY, denom = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    constexpr int AHEAD = 16;
+                    constexpr int AHEAD = 8;
 #pragma unroll 1
                     for (int k0 = 0; k0 < n; k0 += AHEAD) {
                         float2 y[AHEAD];
