@@ -10,8 +10,7 @@
 // all in fp32 with correctly rounded divisions, ties to even.  A value that is not finite makes the scale NaN, and with it
 // every result that reads the page.  Blocks behind those of K and V rotate Q.
 //
-// Bound by bytes for prompts (each value is read once, kept in registers between the maximum and the store, and written
-// once) and by latency for single tokens: offsets, table entry and row are asked for together.
+// Bound by bytes for prompts (each value is read once, for 8-bit pages a second time from L1 or L2, and written once) and by latency for single tokens: offsets, table entry and row are asked for together.
 #pragma once
 
 #include "vteb_common.cuh"
@@ -33,8 +32,6 @@ struct PagedAppendArgs {
     int rope_type, rotary_dim, rope_rows;
     int kv_blocks;                       // blocks of K and V, in front of those of Q
 };
-
-constexpr int kAppendQTasks = 4;         // 16-channel tasks of a thread that rotates Q
 
 #if defined(__CUDACC__)
 
@@ -129,9 +126,12 @@ __device__ __forceinline__ uint2 quantise8(uint4 x, float inv) {
     return make_uint2(narrow4<KIND>(f[0].x, f[0].y, f[1].x, f[1].y), narrow4<KIND>(f[2].x, f[2].y, f[3].x, f[3].y));
 }
 
-// KIND 0: fp16 pages, 1: e4m3, 2: int8.  IT: tasks of a thread, blockDim * IT >= page * D / 16.
-template <int KIND, int IT>
-__global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ PagedAppendArgs p)
+// KIND 0: fp16 pages, 1: e4m3, 2: int8.  Many threads of one 16-channel task each and few registers keep more bytes on their way
+// than several tasks a thread, and for 8-bit pages it is better to read all but a thread's last task a second time, from L1 or L2,
+// than to have fewer threads for the registers that hold them (a 32,768-token prompt of 12 query and 2 KV heads of 128 into e4m3
+// pages: 46 us; with four tasks a thread 52, with all values in registers and five blocks an SM 51).
+template <int KIND>
+__global__ void __launch_bounds__(256, 7) paged_append_kernel(const __grid_constant__ PagedAppendArgs p)
 {
     const int D = 1 << p.dim_log2, tasks_log2 = p.dim_log2 - 4, P = 1 << p.page_log2;
     const int tid = threadIdx.x, T = blockDim.x;
@@ -140,35 +140,31 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
     grid_launch_dependents();
     if ((int)blockIdx.x >= p.kv_blocks) {                   // ---- Q
         const long long all = ((long long)p.total_tokens * p.num_q_heads) << tasks_log2;
-        const long long t0 = (long long)(blockIdx.x - p.kv_blocks) * T * kAppendQTasks + tid;
-#pragma unroll
-        for (int i = 0; i < kAppendQTasks; ++i) {
-            const long long at = t0 + i * T;
-            if (at >= all) break;
-            const int pv = (int)(at & ((1 << tasks_log2) - 1));
-            const int row = (int)(at >> tasks_log2);
-            const int token = row / p.num_q_heads, head = row - token * p.num_q_heads;
-            int b;
-            if (p.token_starts) {
-                int lo = 0, hi = p.batch;                   // the last sequence that starts at or before the token
-                while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (__ldg(p.token_starts + mid) <= token) lo = mid; else hi = mid; }
-                b = lo;
-            } else b = token / p.each;
-            int first, count;
-            token_range(p, b, first, count);
-            const int pos = __ldg(p.kv_offsets + b) - count + 1 + token - first;
-            if (token < first || token >= first + count || pos < 0 || (p.rope_type >= 0 && pos >= p.rope_rows)) continue;
-            const ChannelTask t = channel_task(pv, D, p.rope_type, p.rotary_dim);
-            const __half* src = p.q + token * p.q_stride + head * D;
-            uint4 xa = *reinterpret_cast<const uint4*>(src + t.a), xb = *reinterpret_cast<const uint4*>(src + t.b);
-            if (t.rotated) {
-                const long long e = (long long)pos * (p.rope_type == 2 ? p.rotary_dim : D) + t.entry;
-                rotate_task(t, xa, xb, __ldg(reinterpret_cast<const uint4*>(p.cos_table + e)), __ldg(reinterpret_cast<const uint4*>(p.sin_table + e)));
-            }
-            __half* dst = p.q_out + token * p.q_out_stride + head * D;
-            *reinterpret_cast<uint4*>(dst + t.a) = xa;
-            *reinterpret_cast<uint4*>(dst + t.b) = xb;
+        const long long at = (long long)(blockIdx.x - p.kv_blocks) * T + tid;
+        if (at >= all) return;
+        const int pv = (int)(at & ((1 << tasks_log2) - 1));
+        const int row = (int)(at >> tasks_log2);
+        const int token = row / p.num_q_heads, head = row - token * p.num_q_heads;
+        const ChannelTask t = channel_task(pv, D, p.rope_type, p.rotary_dim);
+        const __half* src = p.q + token * p.q_stride + head * D;
+        uint4 xa = *reinterpret_cast<const uint4*>(src + t.a), xb = *reinterpret_cast<const uint4*>(src + t.b);   // on their way while the position is looked up
+        int b;
+        if (p.token_starts) {
+            int lo = 0, hi = p.batch;                   // the last sequence that starts at or before the token
+            while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (__ldg(p.token_starts + mid) <= token) lo = mid; else hi = mid; }
+            b = lo;
+        } else b = token / p.each;
+        int first, count;
+        token_range(p, b, first, count);
+        const int pos = __ldg(p.kv_offsets + b) - count + 1 + token - first;
+        if (token < first || token >= first + count || pos < 0 || (p.rope_type >= 0 && pos >= p.rope_rows)) return;
+        if (t.rotated) {
+            const long long e = (long long)pos * (p.rope_type == 2 ? p.rotary_dim : D) + t.entry;
+            rotate_task(t, xa, xb, __ldg(reinterpret_cast<const uint4*>(p.cos_table + e)), __ldg(reinterpret_cast<const uint4*>(p.sin_table + e)));
         }
+        __half* dst = p.q_out + token * p.q_out_stride + head * D;
+        *reinterpret_cast<uint4*>(dst + t.a) = xa;
+        *reinterpret_cast<uint4*>(dst + t.b) = xb;
         return;
     }
 
@@ -217,33 +213,42 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
     float* scale_at = KIND == 0 ? nullptr : (is_v ? p.v_scale : p.k_scale) + (long long)page * p.num_kv_heads + h;
     const float old = (KIND != 0 && slot > 0) ? *scale_at : 0.f;
 
-    uint4 xa[IT], xb[IT];
-    uint32_t top = 0;                                       // of the magnitudes' bits, in both halves: NaN is above infinity
-#pragma unroll
-    for (int i = 0; i < IT; ++i) {
-        const int at = tid + i * T, tk = at >> tasks_log2;
-        if (tk >= tokens) continue;
-        const ChannelTask t = channel_task(at & ((1 << tasks_log2) - 1), D, rope, p.rotary_dim);
+    const int tasks = tokens << tasks_log2;
+    auto rotated = [&](int at, ChannelTask& t, uint4& xa, uint4& xb) {
+        const int tk = at >> tasks_log2;
+        t = channel_task(at & ((1 << tasks_log2) - 1), D, rope, p.rotary_dim);
         const __half* row = src + tk * src_stride;
-        xa[i] = *reinterpret_cast<const uint4*>(row + t.a);
-        xb[i] = *reinterpret_cast<const uint4*>(row + t.b);
+        xa = *reinterpret_cast<const uint4*>(row + t.a);
+        xb = *reinterpret_cast<const uint4*>(row + t.b);
         if (t.rotated) {
             const long long e = (long long)(lo + tk) * (rope == 2 ? p.rotary_dim : D) + t.entry;
-            rotate_task(t, xa[i], xb[i], __ldg(reinterpret_cast<const uint4*>(p.cos_table + e)), __ldg(reinterpret_cast<const uint4*>(p.sin_table + e)));
+            rotate_task(t, xa, xb, __ldg(reinterpret_cast<const uint4*>(p.cos_table + e)), __ldg(reinterpret_cast<const uint4*>(p.sin_table + e)));
         }
-        if (KIND == 0) {
-            __half* dst = (__half*)(is_v ? p.v_pool : p.k_pool) + base + (long long)(slot + tk) * p.token_stride;
-            *reinterpret_cast<uint4*>(dst + t.a) = xa[i];
-            *reinterpret_cast<uint4*>(dst + t.b) = xb[i];
-        } else {
-            const uint32_t* a = reinterpret_cast<const uint32_t*>(&xa[i]);
-            const uint32_t* c = reinterpret_cast<const uint32_t*>(&xb[i]);
+        return tk;
+    };
+    if constexpr (KIND == 0) {
+        __half* pool = (__half*)(is_v ? p.v_pool : p.k_pool) + base;
+        for (int at = tid; at < tasks; at += T) {
+            ChannelTask t;
+            uint4 xa, xb;
+            __half* dst = pool + (long long)(slot + rotated(at, t, xa, xb)) * p.token_stride;
+            *reinterpret_cast<uint4*>(dst + t.a) = xa;
+            *reinterpret_cast<uint4*>(dst + t.b) = xb;
+        }
+    } else {
+        __shared__ uint32_t s_top[8];
+        uint32_t top = 0;                                   // of the magnitudes' bits, in both halves: NaN is above infinity
+        ChannelTask t;
+        uint4 xa = make_uint4(0, 0, 0, 0), xb = xa;
+        int tk = 0;
+        const int last = tasks - 1 - tid < 0 ? tid : tid + (tasks - 1 - tid) / T * T;        // a thread's last task, whose values it keeps
+        for (int at = tid; at < tasks; at += T) {
+            tk = rotated(at, t, xa, xb);
+            const uint32_t* a = reinterpret_cast<const uint32_t*>(&xa);
+            const uint32_t* c = reinterpret_cast<const uint32_t*>(&xb);
 #pragma unroll
             for (int k = 0; k < 4; ++k) top = __vmaxu2(top, __vmaxu2(a[k] & 0x7fff7fffu, c[k] & 0x7fff7fffu));
         }
-    }
-    if constexpr (KIND != 0) {
-        __shared__ uint32_t s_top[8];
         top = max(top & 0xffffu, top >> 16);
         top = __reduce_max_sync(~0u, top);
         if ((tid & 31) == 0) s_top[tid >> 5] = top;
@@ -255,14 +260,11 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
         const float inv = now == 0.f ? 0.f : __fdiv_rn(1.f, now);
         if (tid == 0) *scale_at = now;
         unsigned char* pool = (unsigned char*)(is_v ? p.v_pool : p.k_pool) + base;
-#pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            const int at = tid + i * T, tk = at >> tasks_log2;
-            if (tk >= tokens) continue;
-            const ChannelTask t = channel_task(at & ((1 << tasks_log2) - 1), D, rope, p.rotary_dim);
+        for (int at = last; at >= 0 && at < tasks; at -= T) {
+            if (at != last) tk = rotated(at, t, xa, xb);
             unsigned char* dst = pool + (long long)(slot + tk) * p.token_stride;
-            *reinterpret_cast<uint2*>(dst + t.a) = quantise8<KIND>(xa[i], inv);
-            *reinterpret_cast<uint2*>(dst + t.b) = quantise8<KIND>(xb[i], inv);
+            *reinterpret_cast<uint2*>(dst + t.a) = quantise8<KIND>(xa, inv);
+            *reinterpret_cast<uint2*>(dst + t.b) = quantise8<KIND>(xb, inv);
         }
         if (now > old && slot > 0) {                        // the older tokens of the page under the new scale
             const float factor = __fdiv_rn(old, now);

@@ -126,14 +126,6 @@ int launch(void (*fn)(const Args), const Args& args, unsigned grid, unsigned thr
     return report_rt(cudaLaunchKernelEx(&cfg, fn, args), what);
 }
 
-typedef void (*AppendKernel)(const PagedAppendArgs);
-
-template <int KIND>
-AppendKernel append_of(int it) {
-    return it <= 1 ? paged_append_kernel<KIND, 1> : it <= 2 ? paged_append_kernel<KIND, 2>
-         : it <= 4 ? paged_append_kernel<KIND, 4> : paged_append_kernel<KIND, 8>;
-}
-
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
@@ -224,17 +216,18 @@ int vteb_paged_append(const vteb_paged_cache_t* c, const vteb_paged_append_t* a,
     p.total_tokens = a->total_tokens; p.each = a->token_starts ? 0 : a->total_tokens / a->batch;
     p.num_q_heads = a->num_q_heads; p.num_kv_heads = c->num_kv_heads; p.dim_log2 = log2_of(D);
     p.rope_type = a->rope_type; p.rotary_dim = a->rope_type == 2 ? a->rotary_dim : D; p.rope_rows = a->rope_rows;
-    // one thread a 16-channel task of a full page, up to 256 of them
+    // Up to two 16-channel tasks of a full page a thread, in blocks of 128 (256 for pages of 16 KB and more); single tokens leave
+    // most threads of a block idle: 64.
     const int tasks = c->page_size * D / 16;
-    const int threads = tasks < 64 ? 64 : tasks > 256 ? 256 : tasks, it = (tasks + threads - 1) / threads;
+    const int threads = p.each == 1 || tasks < 128 ? 64 : tasks > 512 ? 256 : 128;
     const long long slots = a->token_starts ? (long long)a->total_tokens / c->page_size + 2ll * a->batch
                           : p.each == 1 ? a->batch : (long long)a->batch * (p.each / c->page_size + 2);
     const long long kv_blocks = slots * c->num_kv_heads * 2;
     const long long q_tasks = a->q ? (long long)a->total_tokens * a->num_q_heads * (D / 16) : 0;
-    const long long q_blocks = (q_tasks + (long long)threads * kAppendQTasks - 1) / ((long long)threads * kAppendQTasks);
-    if (kv_blocks + q_blocks > INT_MAX) return report(VTEB_ERR_TOO_LARGE, "%d tokens: too many blocks", a->total_tokens);
+    const long long q_blocks = (q_tasks + threads - 1) / threads;
+    if (kv_blocks + q_blocks > INT_MAX || q_tasks > (1ll << 40)) return report(VTEB_ERR_TOO_LARGE, "%d tokens: too many blocks", a->total_tokens);
     p.kv_blocks = (int)kv_blocks;
-    AppendKernel k = c->type == kPagedF16 ? append_of<0>(it) : c->type == kPagedE4m3 ? append_of<1>(it) : append_of<2>(it);
+    auto k = c->type == kPagedF16 ? paged_append_kernel<0> : c->type == kPagedE4m3 ? paged_append_kernel<1> : paged_append_kernel<2>;
     return launch(k, p, (unsigned)(kv_blocks + q_blocks), threads, 0, stream, (a->launch_flags & VTEB_LAUNCH_PROGRAMMATIC) != 0, "paged append launch");
 }
 
