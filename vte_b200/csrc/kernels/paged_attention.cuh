@@ -45,8 +45,9 @@ struct PagedAttnArgs {
     const int* kv_offsets;           // [batch]
     const float* k_scale;            // [num_pages, Hkv], 8-bit pages
     const float* v_scale;
-    int* counters;                   // [workers], zero between launches: a cut segment's, at its first worker (no two share one)
-    float* part_ml;                  // [2 * workers][rows][2]
+    int* counters;                   // [2][2 * workers], zero between launches: of the pieces that are merged into one
+    float* part_ml;                  // [2 * workers][rows][2]: pieces of cut segments
+    float* part_ml2;                 // the same of merged ones
     float* part_o;                   // [2 * workers][rows][D]
     int* status;
     int batch, max_pages, num_pages, page_log2, box_log2;
@@ -62,6 +63,7 @@ __host__ __device__ constexpr int paged_unit(int row_bytes) { return row_bytes >
 __host__ __device__ constexpr int paged_warps(int row_bytes) { return row_bytes == 512 ? 6 : 8; }
 constexpr int kPagedMaxWorkers = 2;      // of a CTA
 // Measured in paged_attention_kernel, where they are used.
+constexpr int kPagedJoin = 8;            // pieces that are merged at once
 constexpr int kPagedTwoFrom = 4, kPagedAligned = 8, kPagedUnitsOfAWarp = 2;
 
 template <int D, int KIND, int NT>
@@ -754,19 +756,31 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             // the workers whose runs hold units of this segment
             const int begin = hi - at.left - at.first;      // its first unit, of all
             const int w0 = begin / per, w1 = (begin + at.units - 1) / per, n = w1 - w0 + 1;
-            group_barrier(gw, group);
-            if (gt == 0) {
-                __threadfence();                            // for the whole worker: its stores are in front of the barrier
-                const int before = atomicAdd(a.counters + w0, 1);
-                s_last[group] = before == n - 1;
-                if (before == n - 1) a.counters[w0] = 0;    // ready for the next launch
-            }
-            group_barrier(gw, group);
-            if (s_last[group]) {
+            const int p0 = 2 * w0 + (w0 * per == begin ? 0 : 1);
+            auto place = [&](int k) { return k == 0 ? p0 : 2 * (w0 + k); };     // of a piece
+            // Whoever comes last of up to kPagedJoin consecutive pieces merges those in place, and whoever comes last of these merges
+            // them: the many pieces of a long segment are read by several SMs, most of them ahead of the last piece.
+            const int join = n <= kPagedJoin ? n : n <= kPagedJoin * kPagedJoin ? kPagedJoin : (n + kPagedJoin - 1) / kPagedJoin;
+            const int mine_at = (worker - w0) / join * join;
+#pragma unroll 1
+            for (int level = 0; level < 2; ++level) {
+                const int step = level ? join : 1, start = level ? 0 : mine_at;
+                const int count = level ? (n + join - 1) / join : min(join, n - start);
+                const bool done = level || join == n;
+                int* counter = a.counters + (level ? 2 * kPagedMaxWorkers * grid : 0) + place(start);
+                group_barrier(gw, group);
+                if (gt == 0) {
+                    __threadfence();                        // for the whole worker: its stores are in front of the barrier
+                    const bool last = atomicAdd(counter, 1) == count - 1;
+                    s_last[group] = last;
+                    if (last) *counter = 0;                 // ready for the next launch
+                }
+                group_barrier(gw, group);
+                if (!s_last[group]) break;
                 __threadfence();
-                const int p0 = 2 * w0 + (w0 * per == begin ? 0 : 1);
-                // Four columns a thread, the pieces in order: eight reads of each on their way, as they come from L2 (sixteen take registers that the
-                // main loop needs: 16 ragged int8 sequences of 256-wide heads 90 and 95 us).
+                const float2* ml_from = reinterpret_cast<const float2*>(level ? a.part_ml2 : a.part_ml);
+                // Four columns a thread, the pieces in order: eight reads of each on their way, as they come from L2 (sixteen take
+                // registers that the main loop needs: 16 ragged int8 sequences of 256-wide heads 90 and 95 us).
 #pragma unroll 1
                 for (int i = gt; i < rows_here * (D / 4); i += gthreads) {
                     const int row = i / (D / 4), col = i % (D / 4) * 4;
@@ -774,13 +788,13 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
                     constexpr int AHEAD = 8;
 #pragma unroll 1
-                    for (int k0 = 0; k0 < n; k0 += AHEAD) {
+                    for (int k0 = 0; k0 < count; k0 += AHEAD) {
                         float2 y[AHEAD];
                         float4 v[AHEAD];
 #pragma unroll
                         for (int q = 0; q < AHEAD; ++q) {
-                            const int k = min(k0 + q, n - 1), from = (k == 0 ? p0 : 2 * (w0 + k)) * ROWS + row;
-                            y[q] = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + from);
+                            const int from = place(start + min(k0 + q, count - 1) * step) * ROWS + row;
+                            y[q] = __ldcg(ml_from + from);
                             v[q] = __ldcg(reinterpret_cast<const float4*>(a.part_o + from * D + col));
                         }
                         float over = top;
@@ -792,14 +806,21 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                         x.x *= old; x.y *= old; x.z *= old; x.w *= old;
 #pragma unroll
                         for (int q = 0; q < AHEAD; ++q) {
-                            const float f = k0 + q < n ? fast_exp2(y[q].x - ref) : 0.f;
+                            const float f = k0 + q < count ? fast_exp2(y[q].x - ref) : 0.f;
                             denom += y[q].y * f;
                             x.x += v[q].x * f; x.y += v[q].y * f; x.z += v[q].z * f; x.w += v[q].w * f;
                         }
                     }
-                    put(row, col, make_float2(x.x, x.y), top, denom);
-                    put(row, col + 2, make_float2(x.z, x.w), top, denom);
+                    if (done) {
+                        put(row, col, make_float2(x.x, x.y), top, denom);
+                        put(row, col + 2, make_float2(x.z, x.w), top, denom);
+                    } else {                                // only this thread reads what it overwrites
+                        const int to = place(start) * ROWS + row;
+                        *reinterpret_cast<float4*>(a.part_o + to * D + col) = x;
+                        if (col == 0) reinterpret_cast<float2*>(a.part_ml2)[to] = make_float2(top, denom);
+                    }
                 }
+                if (done) break;
             }
         }
         if (!cursor_next_segment<U>(a, at)) break;

@@ -74,10 +74,10 @@ Workspace workspace_of(int rows, int head_dim, int sms) {
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     const size_t workers = (size_t)sms * kPagedMaxWorkers, pieces = 2 * workers;
     Workspace w;
-    w.counters = up(workers * 4);
+    w.counters = up(2 * pieces * 4);
     w.ml = up(pieces * block * 8);
     w.o = up(pieces * block * (size_t)head_dim * 4);
-    w.bytes = w.counters + w.ml + w.o;
+    w.bytes = w.counters + 2 * w.ml + w.o;
     return w;
 }
 
@@ -271,7 +271,8 @@ int vteb_paged_attention(const vteb_paged_cache_t* c, const vteb_paged_attention
     unsigned char* base = (unsigned char*)a->workspace;
     p.counters = (int*)base;
     p.part_ml = (float*)(base + w.counters);
-    p.part_o = (float*)(base + w.counters + w.ml);
+    p.part_ml2 = (float*)(base + w.counters + w.ml);
+    p.part_o = (float*)(base + w.counters + 2 * w.ml);
     p.status = a->status;
     p.batch = a->batch; p.max_pages = a->max_pages; p.num_pages = c->num_pages;
     p.page_log2 = log2_of(c->page_size);
