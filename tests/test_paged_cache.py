@@ -109,6 +109,9 @@ class FakeRuntime:
     def safe_memset(self, p, n, tag):
         assert self.live[p.value] == n
 
+    def synchronize(self):
+        pass
+
     def paged_cache_init(self, cache):
         if self.fail:
             raise CudaSafetyError("refused")

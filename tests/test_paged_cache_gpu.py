@@ -318,6 +318,7 @@ def test_prompt_then_steps_in_a_graph(dev, kind):
     need = PagedKVCache.workspace_bytes(rt, meta, B)
     scratch = rt.safe_malloc(need, "scratch")
     rt.safe_memset(scratch, need)
+    rt.synchronize()
     dtype = np.float16 if kind == "f16" else np.uint8 if kind == "e4m3" else np.int8
     image = [([np.zeros((pages, H, page, D), dtype=dtype) for _ in range(2)], [np.zeros((pages, H), dtype=np.float32) for _ in range(2)]) for _ in range(layers)]
     starts = np.concatenate([[0], np.cumsum(prompts)]).astype(np.int32)
@@ -409,3 +410,134 @@ def test_bad_pages_and_positions_are_reported(dev):
             with pytest.raises(CudaRuntimeError, match="beyond its block table"):
                 rt.synchronize()
         cache.cleanup()
+
+
+def test_nothing_cached(dev):
+    for lengths in ([0], [0, 0, 0]):
+        (out, lse), _ = attend(dev, "e4m3", (8, 2, 128), 16, lengths, queries=2)
+        assert not out.any() and (lse == -np.inf).all()
+
+
+def test_pages_far_into_a_large_pool(dev):
+    """Pools of more than 2^32 values: the pages that are used lie at their ends."""
+    rt = dev.rt
+    rng = np.random.default_rng(21)
+    heads, page, n = (4, 2, 128), 128, 300
+    Hq, H, D = heads
+    pages = (1 << 32) // (H * page * D) + 40
+    cache = PagedKVCache(rt, metadata(heads), pages, page, "e4m3")
+    try:
+        table = np.array([[pages - 1, pages - 3, 131072]], dtype=np.int32)       # the last one begins at 2^32
+        k, v = (rng.standard_normal((n, H, D), dtype=np.float32).astype(np.float16) for _ in range(2))
+        q = rng.standard_normal((1, 1, Hq, D), dtype=np.float32).astype(np.float16)
+        offsets = np.array([n - 1], dtype=np.int32)
+        d_table, d_off, d_out = dev.put(table), dev.put(offsets), dev.put(q)
+        cache.append(dev.put(k), dev.put(v), d_table, d_off, 1, 3, total_tokens=n)
+        cache.attend(dev.put(q), d_out, d_table, d_off, 1, 3)
+        rt.synchronize()
+        small = np.array([[0, 1, 2]], dtype=np.int32)
+        pools, scales = [np.zeros((3, H, page, D), dtype=np.uint8) for _ in range(2)], [np.zeros((3, H), dtype=np.float32) for _ in range(2)]
+        orc.append(pools, scales, "e4m3", (k, v), small, offsets, [0, n], page)
+        for ptr, pool in ((cache.k_pool, pools[0]), (cache.v_pool, pools[1])):
+            for i, at in enumerate(table[0]):
+                rows = min(page, n - i * page)
+                got = dev.get(ptr + int(at) * H * page * D, pool[i])
+                assert np.array_equal(got[:, :rows], pool[i][:, :rows])
+        ref, _, bound = orc.attention(q, *pools, *scales, "e4m3", small, offsets, 1.0 / np.sqrt(D))
+        assert (np.abs(dev.get(d_out, q) - ref) <= tolerance(bound, ref, D, False)).all()
+    finally:
+        cache.cleanup()
+
+
+def test_one_pool_for_k_and_v_and_pages_that_sequences_share(dev):
+    """K and V of a page side by side in one pool, and a prefix whose pages are two sequences'."""
+    rng = np.random.default_rng(22)
+    heads, page = (6, 3, 64), 32
+    Hq, H, D = heads
+    lengths = np.array([70, 90])
+    pages = 6
+    table = np.array([[4, 2, 0], [4, 2, 5]], dtype=np.int32)
+    both = rng.standard_normal((pages, 2, H, page, D), dtype=np.float32).astype(np.float16)
+    at = dev.put(both)
+    cache = PagedKVCache(dev.rt, metadata(heads), pages, page, "f16", k_pool=at, v_pool=at + H * page * D * 2,
+                         strides=(2 * H * page * D, D, page * D))
+    q = rng.standard_normal((2, 1, Hq, D), dtype=np.float32).astype(np.float16)
+    d_out, offsets = dev.put(q), (lengths - 1).astype(np.int32)
+    cache.attend(dev.put(q), d_out, dev.put(table), dev.put(offsets), 2, 3)
+    dev.rt.synchronize()
+    ref, _, bound = orc.attention(q, both[:, 0], both[:, 1], None, None, "f16", table, offsets, 1.0 / np.sqrt(D))
+    assert (np.abs(dev.get(d_out, q) - ref) <= tolerance(bound, ref, D, False)).all()
+    cache.cleanup()
+
+
+def test_another_stream_and_a_workspace_for_all_shapes(dev):
+    """Calls of different shapes one behind the other on a stream of the caller's, all with one workspace, which each of them
+    leaves ready for the next."""
+    rt = dev.rt
+    rng = np.random.default_rng(23)
+    stream = ctypes.c_void_p()
+    assert rt._lib.vteb_stream_create(ctypes.byref(stream)) == 0
+    shapes = [((12, 2, 128), 16, [3000]), ((32, 8, 64), 64, [10, 700, 0, 90, 5000]), ((8, 2, 256), 32, [2500, 40]), ((12, 2, 128), 16, [200] * 90)]
+    need = max(PagedKVCache.workspace_bytes(rt, metadata(h), len(n), 4) for h, _, n in shapes)
+    scratch = rt.safe_malloc(need, "scratch")
+    rt.safe_memset(scratch, need)
+    rt.synchronize()
+    runs = []
+    for heads, page, lengths in shapes + shapes[::-1]:
+        kind = ("f16", "e4m3", "int8")[len(runs) % 3]
+        table, pages = table_of(rng, lengths, page)
+        pools, scales = zip(*(random_pool(rng, kind, pages, heads, page) for _ in range(2)))
+        cache, _, _ = make_cache(dev, metadata(heads), kind, page, pools, scales)
+        queries = 1 + len(runs) % 3
+        q = rng.standard_normal((len(lengths), queries, heads[0], heads[2]), dtype=np.float32).astype(np.float16)
+        offsets = np.asarray(lengths, dtype=np.int32) - 1
+        d_out = dev.put(np.zeros_like(q))
+        args = (dev.put(q), d_out, dev.put(table), dev.put(offsets), len(lengths), table.shape[1])
+        runs.append((cache, args, queries, q, d_out, (pools, scales, kind, table, offsets), heads))
+    for cache, args, queries, *_ in runs:
+        cache.attend(*args, query_tokens=queries, workspace=scratch, workspace_bytes=need, stream=stream.value)
+    rt.synchronize()
+    for cache, _, _, q, d_out, (pools, scales, kind, table, offsets), heads in runs:
+        ref, _, bound = orc.attention(q, *pools, *scales, kind, table, offsets, 1.0 / np.sqrt(heads[2]))
+        assert (np.abs(dev.get(d_out, q) - ref) <= tolerance(bound, ref, heads[2], False)).all()
+        cache.cleanup()
+    with pytest.raises(CudaSafetyError, match="workspace holds"):
+        runs[0][0].attend(*runs[0][1], workspace=scratch, workspace_bytes=1000)
+    rt.safe_free(scratch)
+    assert rt._lib.vteb_stream_destroy(stream) == 0
+
+
+def test_two_graphs_on_two_streams(dev):
+    """Two captured steps, each with its cache and its workspace, replayed on two streams at once."""
+    rt = dev.rt
+    rng = np.random.default_rng(24)
+    heads, page = (12, 2, 128), 64
+    steps = []
+    for n in (9000, 12000):
+        table, pages = table_of(rng, [n], page)
+        pools, scales = zip(*(random_pool(rng, "e4m3", pages, heads, page) for _ in range(2)))
+        cache, _, _ = make_cache(dev, metadata(heads), "e4m3", page, pools, scales)
+        cache.reserve(1)
+        q = rng.standard_normal((1, 1, heads[0], heads[2]), dtype=np.float32).astype(np.float16)
+        offsets = np.array([n - 1], dtype=np.int32)
+        d_out = dev.put(np.zeros_like(q))
+        args = (dev.put(q), d_out, dev.put(table), dev.put(offsets), 1, table.shape[1])
+        rt.synchronize()
+        rt.stream_begin_capture()
+        for _ in range(8):
+            cache.attend(*args)
+        graph = rt.stream_end_capture()
+        stream = ctypes.c_void_p()
+        assert rt._lib.vteb_stream_create(ctypes.byref(stream)) == 0
+        steps.append((rt.graph_instantiate(graph), stream, cache, q, d_out, (pools, scales, table, offsets)))
+        rt.graph_destroy(graph)
+    for _ in range(20):
+        for step, stream, *_ in steps:
+            assert rt._lib.vteb_graph_launch(step, stream) == 0
+    rt.synchronize()
+    for step, stream, cache, q, d_out, (pools, scales, table, offsets) in steps:
+        ref, _, bound = orc.attention(q, *pools, *scales, "e4m3", table, offsets, 1.0 / np.sqrt(128))
+        assert (np.abs(dev.get(d_out, q) - ref) <= tolerance(bound, ref, 128, False)).all()
+        rt.graph_exec_destroy(step)
+        cache.cleanup()
+        assert rt._lib.vteb_stream_destroy(stream) == 0

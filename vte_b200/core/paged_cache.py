@@ -33,8 +33,7 @@ def _heads(metadata):
 
 class PagedKVCache:
     """`k_pool`, `v_pool` (and `k_scale`, `v_scale`): the caller's memory, with `strides` (page, token, head, in values);
-    without pools they are allocated, from `allocator` where one is given, with the positions of a head side by side.
-    `workspace` is the scratch of `attend`; without one it is allocated for `batch_size` sequences of up to `query_tokens`."""
+    without pools they are allocated, from `allocator` where one is given, with the positions of a head side by side."""
 
     def __init__(self, hip, metadata, num_pages: int, page_size: int = 64, cache_type: str = "f16", *, k_pool=0, v_pool=0,
                  k_scale=0, v_scale=0, strides=None, allocator=None):
@@ -97,6 +96,7 @@ class PagedKVCache:
             self._owned.append(handle)
             ptr = handle.value
         self.hip.safe_memset(ctypes.c_void_p(ptr), size, tag)
+        self.hip.synchronize()                    # calls may come on any stream
         return ptr
 
     @staticmethod
@@ -153,7 +153,9 @@ class PagedKVCache:
         self.hip.paged_attention(self._cache, a, stream)
 
     def cleanup(self) -> None:
-        """Frees what this cache allocated."""
+        """Frees what this cache allocated (a runtime that has been cleaned up has done so already)."""
+        if self._allocator is None and not getattr(self.hip, "_initialized", True):
+            self._owned.clear()
         for block in self._owned:
             if self._allocator is not None:
                 self._allocator.free(block)

@@ -258,13 +258,13 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
     // Workers of a CTA: two where there are segments for them, so that one computes while the other merges (64 sequences of
     // 8 x 64-wide e4m3 heads: 114 us with one, 103 with two, 104 with four); one where few segments would be cut more often
     // for that (32,768 positions of 2 x 128-wide e4m3 heads: 15 and 19 us).
-    const int segments = lives * HR, grid = gridDim.x;
+    const int segments = max(lives * HR, 1), grid = gridDim.x;      // (1 where nothing is cached: no worker has a unit then)
     const int groups = segments * kPagedTwoFrom >= grid ? kPagedMaxWorkers : 1, workers = grid * groups;
     const int gw = W / groups, group = groups == 1 ? 0 : warp / (W / 2), wi = groups == 1 ? warp : warp % (W / 2);
     // Units of a worker: an equal share, but not so few that a segment is cut where its warps would have little to do each.
     // Short runs begin with a segment each: `per` units stand for what is left of one, so that no worker has parts of two.
     const bool aligned = segments * 2 <= workers && total < workers * gw * kPagedAligned;
-    const int mean = segments ? (total + segments - 1) / segments : 1, cuts = (mean + kPagedUnitsOfAWarp * gw - 1) / (kPagedUnitsOfAWarp * gw);
+    const int mean = max((total + segments - 1) / segments, 1), cuts = (mean + kPagedUnitsOfAWarp * gw - 1) / (kPagedUnitsOfAWarp * gw);
     const int over = !aligned ? workers : a.batch == 1 ? workers / segments * segments : workers - segments;
     const int per = max((total + over - 1) / over, (mean + cuts - 1) / cuts);
     auto room_of = [&](int units) { return aligned ? (units + per - 1) / per * per : units; };
