@@ -31,6 +31,7 @@ struct PagedAppendArgs {
     int num_q_heads, num_kv_heads, dim_log2;
     int rope_type, rotary_dim, rope_rows;
     int kv_blocks;                       // blocks of K and V, in front of those of Q
+    int q_heads_each;                    // heads of Q a thread, a divisor of num_q_heads
 };
 
 #if defined(__CUDACC__)
@@ -126,12 +127,12 @@ __device__ __forceinline__ uint2 quantise8(uint4 x, float inv) {
     return make_uint2(narrow4<KIND>(f[0].x, f[0].y, f[1].x, f[1].y), narrow4<KIND>(f[2].x, f[2].y, f[3].x, f[3].y));
 }
 
-// KIND 0: fp16 pages, 1: e4m3, 2: int8.  Many threads of one 16-channel task each and few registers keep more bytes on their way
-// than several tasks a thread, and for 8-bit pages it is better to read all but a thread's last task a second time, from L1 or L2,
-// than to have fewer threads for the registers that hold them (a 32,768-token prompt of 12 query and 2 KV heads of 128 into e4m3
-// pages: 46 us; with four tasks a thread 52, with all values in registers and five blocks an SM 51).
+// KIND 0: fp16 pages, 1: e4m3, 2: int8.  One 16-channel task of K and V a thread at a time and two of Q, whose position, table rows
+// and conversions are then looked up once; 8-bit pages read all but a thread's last task a second time, from L1 or L2, rather than
+// hold them.  Registers without spills come before more blocks an SM.  A 32,768-token prompt of 12 query and 2 KV heads of 128 into
+// e4m3 pages: 46.5 us; 54.5 with seven blocks of spilling threads, 48.4 with one task of Q a thread, 52 with four.
 template <int KIND>
-__global__ void __launch_bounds__(256, 7) paged_append_kernel(const __grid_constant__ PagedAppendArgs p)
+__global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_constant__ PagedAppendArgs p)
 {
     const int D = 1 << p.dim_log2, tasks_log2 = p.dim_log2 - 4, P = 1 << p.page_log2;
     const int tid = threadIdx.x, T = blockDim.x;
@@ -139,32 +140,45 @@ __global__ void __launch_bounds__(256, 7) paged_append_kernel(const __grid_const
     grid_dependency_wait();
     grid_launch_dependents();
     if ((int)blockIdx.x >= p.kv_blocks) {                   // ---- Q
-        const long long all = ((long long)p.total_tokens * p.num_q_heads) << tasks_log2;
+        // the same sixteen channels of `q_heads_each` heads of a token: one look at its position and its table rows
+        const int groups = p.num_q_heads / p.q_heads_each;
+        const long long all = ((long long)p.total_tokens * groups) << tasks_log2;
         const long long at = (long long)(blockIdx.x - p.kv_blocks) * T + tid;
         if (at >= all) return;
-        const int pv = (int)(at & ((1 << tasks_log2) - 1));
-        const int row = (int)(at >> tasks_log2);
-        const int token = row / p.num_q_heads, head = row - token * p.num_q_heads;
+        const int pv = (int)at & ((1 << tasks_log2) - 1);
+        const unsigned row = (unsigned)(at >> tasks_log2), token = row / (unsigned)groups;
+        const int head = (row - token * groups) * p.q_heads_each;
         const ChannelTask t = channel_task(pv, D, p.rope_type, p.rotary_dim);
         const __half* src = p.q + token * p.q_stride + head * D;
         uint4 xa = *reinterpret_cast<const uint4*>(src + t.a), xb = *reinterpret_cast<const uint4*>(src + t.b);   // on their way while the position is looked up
         int b;
         if (p.token_starts) {
             int lo = 0, hi = p.batch;                   // the last sequence that starts at or before the token
-            while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (__ldg(p.token_starts + mid) <= token) lo = mid; else hi = mid; }
+            while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (__ldg(p.token_starts + mid) <= (int)token) lo = mid; else hi = mid; }
             b = lo;
-        } else b = token / p.each;
+        } else b = p.each == 1 ? token : token / p.each;
         int first, count;
         token_range(p, b, first, count);
-        const int pos = __ldg(p.kv_offsets + b) - count + 1 + token - first;
-        if (token < first || token >= first + count || pos < 0 || (p.rope_type >= 0 && pos >= p.rope_rows)) return;
+        const int pos = __ldg(p.kv_offsets + b) - count + 1 + (int)token - first;
+        if ((int)token < first || (int)token >= first + count || pos < 0 || (p.rope_type >= 0 && pos >= p.rope_rows)) return;
+        uint4 c = make_uint4(0, 0, 0, 0), s = c;
         if (t.rotated) {
             const long long e = (long long)pos * (p.rope_type == 2 ? p.rotary_dim : D) + t.entry;
-            rotate_task(t, xa, xb, __ldg(reinterpret_cast<const uint4*>(p.cos_table + e)), __ldg(reinterpret_cast<const uint4*>(p.sin_table + e)));
+            c = __ldg(reinterpret_cast<const uint4*>(p.cos_table + e));
+            s = __ldg(reinterpret_cast<const uint4*>(p.sin_table + e));
         }
         __half* dst = p.q_out + token * p.q_out_stride + head * D;
-        *reinterpret_cast<uint4*>(dst + t.a) = xa;
-        *reinterpret_cast<uint4*>(dst + t.b) = xb;
+#pragma unroll 1
+        for (int h = 0;;) {
+            if (t.rotated) rotate_task(t, xa, xb, c, s);
+            *reinterpret_cast<uint4*>(dst + t.a) = xa;
+            *reinterpret_cast<uint4*>(dst + t.b) = xb;
+            if (++h == p.q_heads_each) break;
+            src += D;
+            dst += D;
+            xa = *reinterpret_cast<const uint4*>(src + t.a);
+            xb = *reinterpret_cast<const uint4*>(src + t.b);
+        }
         return;
     }
 

@@ -223,7 +223,10 @@ int vteb_paged_append(const vteb_paged_cache_t* c, const vteb_paged_append_t* a,
     const long long slots = a->token_starts ? (long long)a->total_tokens / c->page_size + 2ll * a->batch
                           : p.each == 1 ? a->batch : (long long)a->batch * (p.each / c->page_size + 2);
     const long long kv_blocks = slots * c->num_kv_heads * 2;
-    const long long q_tasks = a->q ? (long long)a->total_tokens * a->num_q_heads * (D / 16) : 0;
+    // One head of Q a thread while that leaves SMs without threads, else two.
+    p.q_heads_each = a->q && a->num_q_heads % 2 == 0 && (long long)a->total_tokens * a->num_q_heads * (D / 16) > (1ll << 19) ? 2 : 1;
+    const int q_groups = a->q ? a->num_q_heads / p.q_heads_each : 1;
+    const long long q_tasks = a->q ? (long long)a->total_tokens * q_groups * (D / 16) : 0;
     const long long q_blocks = (q_tasks + threads - 1) / threads;
     if (kv_blocks + q_blocks > INT_MAX || q_tasks > (1ll << 40)) return report(VTEB_ERR_TOO_LARGE, "%d tokens: too many blocks", a->total_tokens);
     p.kv_blocks = (int)kv_blocks;
