@@ -123,7 +123,7 @@ def attention(q, k_pool, v_pool, k_scale, v_scale, kind, block_table, kv_offsets
                 out[b, i, h] = p @ v[:m, kv] / p.sum()
                 lse[b, i, h] = top + np.log(p.sum())
                 mean[b, i, h] = p @ np.abs(v[:m, kv]) / p.sum()
-                reach[b, i, h] = (np.abs(k[:m, kv]) @ np.abs(q[b, i, h].astype(np.float64))).max() * scale
-                largest = 1.0 if kind == "f16" else v_scale[pages[:-(-m // P)], kv].max()
+                reach[b, i, h] = (np.abs(k[:m, kv]) @ np.abs(q[b, i, h].astype(np.float64))).max() * abs(scale)
+                largest = 1.0 if kind == "f16" else np.abs(v_scale[pages[:-(-m // P)], kv]).max()
                 floor[b, i, h] = stored[:m, kv].sum(axis=0) * largest / p.sum()
     return out, lse, (mean, reach, floor)

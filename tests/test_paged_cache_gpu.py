@@ -135,25 +135,31 @@ def test_what_a_row_does_not_see_does_not_reach_it(dev, kind):
 
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
 def test_scales_of_very_different_size(dev, kind):
-    """Scales from 1e-30 to 1e20 beside each other, and pages of zeros with a scale of zero."""
+    """Scales from 1e-30 to 1e20 beside each other, of both signs, and pages of zeros with a scale of zero; then negative ones alone."""
     rng = np.random.default_rng(9)
     heads, page, n = (8, 2, 64), 16, 400
     table, pages = table_of(rng, [n], page)
     pools, scales = map(list, zip(*(random_pool(rng, kind, pages, heads, page) for _ in range(2))))
     scales[1] = (10.0 ** rng.uniform(-30, 20, size=scales[1].shape)).astype(np.float32)
+    scales[1] *= rng.choice(np.array([-1, 1], dtype=np.float32), size=scales[1].shape)
     zero = table[0, 3]
     for x, s in zip(pools, scales):
         x[zero], s[zero] = 0, 0
-    cache, _, _ = make_cache(dev, metadata(heads), kind, page, pools, scales)
     q = rng.standard_normal((1, 1, heads[0], heads[2]), dtype=np.float32).astype(np.float16)
-    out, offsets = np.zeros(q.shape, dtype=np.float32), np.array([n - 1], dtype=np.int32)
-    d_out = dev.put(out)
-    cache.attend(dev.put(q), d_out, dev.put(table), dev.put(offsets), 1, table.shape[1], output_f32=True)
-    dev.rt.synchronize()
-    out = dev.get(d_out, out)
-    cache.cleanup()
-    ref, _, bound = orc.attention(q, *pools, *scales, kind, table, offsets, 1.0 / 8)
-    assert (np.abs(out - ref) <= tolerance(bound, ref, 64, True)).all()
+    offsets = np.array([n - 1], dtype=np.int32)
+    for negative in (False, True):
+        if negative:
+            scales[1] = -np.abs(scales[1][::-1]).clip(1e-3, 1e3)
+            scales[0] = -scales[0]
+        cache, _, _ = make_cache(dev, metadata(heads), kind, page, pools, scales)
+        out = np.zeros(q.shape, dtype=np.float32)
+        d_out = dev.put(out)
+        cache.attend(dev.put(q), d_out, dev.put(table), dev.put(offsets), 1, table.shape[1], output_f32=True)
+        dev.rt.synchronize()
+        out = dev.get(d_out, out)
+        cache.cleanup()
+        ref, _, bound = orc.attention(q, *pools, *scales, kind, table, offsets, 1.0 / 8)
+        assert (np.abs(out - ref) <= tolerance(bound, ref, 64, True)).all()
 
 
 # ---- append ------------------------------------------------------------------------------------------------------------

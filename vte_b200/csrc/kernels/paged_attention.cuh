@@ -66,9 +66,9 @@ struct PagedAttnArgs {
 __host__ __device__ constexpr int paged_unit(int row_bytes) { return row_bytes >= 256 ? 16 : 4096 / row_bytes; }
 __host__ __device__ constexpr int paged_warps(int row_bytes) { return row_bytes == 512 ? 6 : 8; }
 constexpr int kPagedMaxWorkers = 2;      // of a CTA
-// Two workers a CTA from one segment on every fourth SM (kPagedTwoFrom = 4: four query tokens of 8 sequences of 8 x 128-wide e4m3 heads 30.3 us, 32.4 with one segment an SM
-// on); up to so many units a warp runs begin with a segment (8: the same 30.3 us, 31.7 up to 4); units that a warp of a worker has
-// at least (2: 2,000 positions of 2 x 128-wide heads 10.3 us, 11.7 with 3 and 13.0 with 4).
+// Two workers a CTA from one segment on every fourth SM on (four query tokens of 8 sequences of 8 x 128-wide e4m3 heads 30.3 us, 32.4
+// from one an SM on); runs begin with a segment each up to so many units a warp (the same 30.3 us, 31.7 up to 4); units that a
+// warp of a worker has at least (2,000 positions of 2 x 128-wide heads 10.3 us, 11.7 with 3 and 13.0 with 4).
 constexpr int kPagedJoin = 8;            // pieces that are merged at once (sixteen: 8,000 positions of 2 x 256-wide fp16 heads 14.8 us instead of 13.8)
 constexpr int kPagedTwoFrom = 4, kPagedAligned = 8, kPagedUnitsOfAWarp = 2;
 
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                     for (int sl = 0; sl < SLABS; ++sl) {
                         if (u * U + sl * 16 >= at.len) vs[sl] = 0.f;             // a page behind the last one
                         if (!(fabsf(vs[sl]) < INFINITY)) vs[sl] = NAN;
-                        top = fmaxf(top, vs[sl]);
+                        top = fmaxf(top, fabsf(vs[sl]));
                     }
                     // (steps of 2^64 keep the reciprocal in the normal range)
                     const float step = top > 1.f ? 0x1p-64f : 0x1p64f, inv = top > 0.f ? __fdividef(1.f, top * step) : 0.f;
