@@ -182,36 +182,46 @@ def test_e4m3_grid_and_rounding():
     assert orc.to_e4m3(np.float32(1e9)) == 126 and orc.to_e4m3(np.float32(np.nan)) & 127 == 127
 
 
-def worker_runs(lengths, head_rows, unit, grid, groups, warps):
-    """The runs of units that paged_attention_kernel deals to its workers, as (units of a run, total, [(lo, hi)])."""
-    total = sum(-(-int(n) // unit) for n in lengths) * head_rows
-    per = max(-(-total // (grid * groups)), 2 * (warps // groups))
-    return per, total, [(lo, min(lo + per, total)) for lo in range(0, total, per)]
+def worker_runs(lengths, head_rows, unit, grid, groups, warps, end=2):
+    """The runs that paged_attention_kernel deals to its workers where they are long: equal shares of all units, the end of a
+    segment counted as `end` units a warp.  (units of a run, what a segment's end counts, [[(first, end) by segment]])."""
+    extra = end * (warps // groups)
+    counts = [-(-int(n) // unit) for n in lengths for _ in range(head_rows) if n]
+    total = sum(n + extra for n in counts)
+    mean = max(-(-sum(counts) // max(len(counts), 1)), 1)
+    cuts = -(-mean // extra)
+    per = max(-(-total // (grid * groups)), -(-mean // cuts))
+    begins = np.cumsum([0] + [n + extra for n in counts])
+    return per, begins, counts, -(-total // per)
 
 
-@pytest.mark.parametrize("groups", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("groups", [1, 2])
 def test_pieces_of_cut_segments_have_places_of_their_own(groups):
-    """The kernel's arithmetic for segments that worker borders cut: first and last worker, the piece each one leaves and the
-    counter they share."""
+    """The kernel's arithmetic for segments that worker borders cut: every unit is one worker's, first and last worker of a
+    segment, the piece each one leaves, and the counters of pieces that are merged into one, in two steps where they are many."""
     rng = np.random.default_rng(groups)
     for _ in range(60):
-        lengths = rng.integers(0, rng.choice([40, 500, 9000]), size=rng.integers(1, 40))
-        head_rows, unit = int(rng.choice([1, 2, 8])), int(rng.choice([16, 32, 64]))
-        per, total, runs = worker_runs(lengths, head_rows, unit, 148, groups, 16)
-        assert len(runs) <= 148 * groups and all(lo < hi for lo, hi in runs)
-        begin, pieces, counters = 0, set(), set()
-        for n in lengths:
-            for _ in range(head_rows if n else 0):
-                units = -(-int(n) // unit)
-                owners = [w for w, (lo, hi) in enumerate(runs) if lo < begin + units and hi > begin]
-                w0, w1 = begin // per, (begin + units - 1) // per
-                assert owners == list(range(w0, w1 + 1))
-                if len(owners) > 1:
-                    assert w0 not in counters
-                    counters.add(w0)
-                    for k, w in enumerate(owners):
-                        place = 2 * w + (0 if runs[w][0] >= begin else 1)          # as the worker writes it
-                        assert place == (2 * w0 + (0 if w0 * per == begin else 1) if k == 0 else 2 * w)   # as it is read
-                        assert place not in pieces
-                        pieces.add(place)
-                begin += units
+        lengths = rng.integers(0, rng.choice([40, 500, 9000, 200000]), size=rng.integers(1, 40))
+        head_rows, unit, warps = int(rng.choice([1, 2, 8])), int(rng.choice([16, 32, 64])), int(rng.choice([6, 8]))
+        per, begins, counts, workers = worker_runs(lengths, head_rows, unit, 148, groups, warps)
+        assert workers <= 148 * groups
+        pieces, counters = set(), [set(), set()]
+        for begin, units in zip(begins.tolist(), counts):
+            w0, w1 = begin // per, (begin + units - 1) // per
+            owned = [(max(w * per, begin), min((w + 1) * per, begin + units)) for w in range(w0, w1 + 1)]
+            assert owned[0][0] == begin and owned[-1][1] == begin + units and all(lo < hi for lo, hi in owned)
+            assert all(a[1] == b[0] for a, b in zip(owned, owned[1:]))
+            n = w1 - w0 + 1
+            if n == 1:
+                continue
+            place = [2 * (w0 + k) if k else 2 * w0 + (0 if w0 * per == begin else 1) for k in range(n)]      # as it is read
+            written = [2 * w + (0 if owned[w - w0][0] == w * per else 1) for w in range(w0, w1 + 1)]
+            assert place == written and not pieces & set(place)
+            pieces |= set(place)
+            join = n if n <= 8 else 8 if n <= 64 else -(-n // 8)
+            firsts = list(range(0, n, join))
+            assert len(firsts) <= 8 and all((k // join * join) in firsts for k in range(n))
+            at = [place[k] for k in firsts], [place[0]] if join < n else []
+            for level in (0, 1):
+                assert not counters[level] & set(at[level])
+                counters[level] |= set(at[level])
