@@ -10,7 +10,8 @@
 // all in fp32 with correctly rounded divisions, ties to even.  A value that is not finite makes the scale NaN, and with it
 // every result that reads the page.  Blocks behind those of K and V rotate Q.
 //
-// Bound by bytes for prompts (each value is read once, for 8-bit pages a second time from L1 or L2, and written once) and by latency for single tokens: offsets, table entry and row are asked for together.
+// Bound by bytes and instructions for prompts (each value is read once, for 8-bit pages a second time from L1 or L2, and written
+// once), by latency for single tokens.
 #pragma once
 
 #include "vteb_common.cuh"

@@ -70,7 +70,7 @@ constexpr int kPagedMaxWorkers = 2;      // of a CTA
 // from one an SM on); runs begin with a segment each up to so many units a warp (the same 30.3 us, 31.7 up to 4); units that a
 // warp of a worker has at least (2,000 positions of 2 x 128-wide heads 10.3 us, 11.7 with 3 and 13.0 with 4).
 constexpr int kPagedJoin = 8;            // pieces that are merged at once (sixteen: 8,000 positions of 2 x 256-wide fp16 heads 14.8 us instead of 13.8)
-constexpr int kPagedTwoFrom = 4, kPagedAligned = 8, kPagedUnitsOfAWarp = 2, kPagedSegmentEnd = 2;
+constexpr int kPagedTwoFrom = 4, kPagedTwoBelow = 192, kPagedAligned = 8, kPagedUnitsOfAWarp = 2, kPagedSegmentEnd = 2;
 
 template <int D, int KIND, int NT>
 struct PagedShape {
@@ -262,16 +262,18 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
         for (int w = 0; w < W; ++w) lives += s_live[w];
     }
     total *= HR;
-    // Workers of a CTA: two where there are segments for them, so that one computes while the other merges (64 sequences of
-    // 8 x 64-wide e4m3 heads: 114 us with one, 103 with two, 104 with four); one where few segments would be cut more often
-    // for that (32,768 positions of 2 x 128-wide e4m3 heads: 15 and 19 us).
+    // Workers of a CTA: two where there are segments for them and these are short, so that one computes while the other merges;
+    // one where few segments would be cut more often for that, or where merges are rare beside units (one and two workers: 64
+    // sequences of 8 x 64-wide heads, 136 units of e4m3 each, 100.1 and 96.7 us, 272 units of fp16 each, 151 and 155;
+    // 100 of 10 to 8,000 positions 94 and 86; one of 32,768 positions 12.8 and 14.9).
     const int segments = max(lives * HR, 1), grid = gridDim.x;      // (1 where nothing is cached: no worker has a unit then)
-    const int groups = segments * kPagedTwoFrom >= grid ? kPagedMaxWorkers : 1, workers = grid * groups;
+    const int mean = max((total + segments - 1) / segments, 1);
+    const int groups = segments * kPagedTwoFrom >= grid && mean < kPagedTwoBelow ? kPagedMaxWorkers : 1, workers = grid * groups;
     const int gw = W / groups, group = groups == 1 ? 0 : warp / (W / 2), wi = groups == 1 ? warp : warp % (W / 2);
     // Units of a worker: an equal share, but not so few that a segment is cut where its warps would have little to do each.
     // Short runs begin with a segment each: `per` units stand for what is left of one, so that no worker has parts of two.
     const bool aligned = segments * 2 <= workers && total < workers * gw * kPagedAligned;
-    const int mean = max((total + segments - 1) / segments, 1), cuts = (mean + kPagedUnitsOfAWarp * gw - 1) / (kPagedUnitsOfAWarp * gw);
+    const int cuts = (mean + kPagedUnitsOfAWarp * gw - 1) / (kPagedUnitsOfAWarp * gw);
     const int over = !aligned ? workers : a.batch == 1 ? workers / segments * segments : workers - segments;
     // Long runs count the end of a segment, at which a worker's warps wait for one another, as units too, kPagedSegmentEnd a warp:
     // else runs of many short segments take half as long again as runs of one (100 sequences of 10 to 8,000 positions of
