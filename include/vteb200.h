@@ -318,8 +318,8 @@ int vteb_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_ca
 /* ---- paged caches --------------------------------------------------------
  * A cache as a pool of pages of `page_size` positions (16, 32, 64 or 128).  A block table int32[batch, max_pages] says
  * which pages hold a sequence's positions, in order; kv_offsets int32[batch] is the position of its newest token, as for
- * the contiguous caches, and -1 where a row of the batch is padding.  All of them are device memory; entries of the table
- * behind a sequence's last page are not read.  No counterpart in the reference.
+ * the contiguous caches, and -1 where a row of the batch is padding.  All of them are device memory that does
+ * not change while a call runs; entries of the table behind a sequence's last page are not read.  No counterpart in the reference.
  *
  * Types of the pages.  VTEB_PAGED_F16 holds fp16.  VTEB_PAGED_E4M3 and VTEB_PAGED_INT8 hold 8-bit values with one fp32
  * scale for every page and KV head, of K and of V (k_scale, v_scale fp32[num_pages, num_kv_heads]): a stored value stands
