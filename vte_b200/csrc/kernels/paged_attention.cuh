@@ -18,8 +18,10 @@
 // delivers pairs of values; the order of channels inside a 16-channel step is free as long as Q (or the output column)
 // follows, so K needs no shuffling at all and V one byte permute per four values.  e4m3 and int8 values are exact in
 // fp16.  P is rounded to fp16 where the output is fp16, whose own rounding is as large; for fp32 output it is split into
-// two fp16 parts.  Page scales never touch the stored values: ks multiplies the scores, and O is held in units of the last
-// page's vs, so that P itself is what fp16 has to hold.
+// two fp16 parts.  Weights are taken relative to the row's maximum less kPagedShift, so that fp16 holds those down to 2^-29 of the
+// largest with all its bits and the last ones to 2^-40: relative to the maximum itself, positions 17 above the others took
+// 0.8 % of what those add up to, 5 to 14 % beside pages of larger scales.  Page scales never touch the stored values: ks
+// multiplies the scores, and O is held in units of the last page's vs, so that P itself is what fp16 has to hold.
 //
 // Merging.  A segment's warps are merged through shared memory in warp order.  Segments that a worker border cuts leave
 // (m, l, o) pieces in the workspace, and the last worker to arrive merges them in worker order: results do not depend on
@@ -71,6 +73,8 @@ constexpr int kPagedMaxWorkers = 2;      // of a CTA
 // warp of a worker has at least (2,000 positions of 2 x 128-wide heads 10.3 us, 11.7 with 3 and 13.0 with 4).
 constexpr int kPagedJoin = 8;            // pieces that are merged at once (sixteen: 8,000 positions of 2 x 256-wide fp16 heads 14.8 us instead of 13.8)
 constexpr int kPagedTwoFrom = 4, kPagedTwoBelow = 192, kPagedAligned = 8, kPagedUnitsOfAWarp = 2, kPagedSegmentEnd = 2;
+
+constexpr float kPagedShift = 15.f, kPagedUnshift = 0x1p-15f;     // 2^15 is the largest power of two that fp16 has
 
 template <int D, int KIND, int NT>
 struct PagedShape {
@@ -395,6 +399,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
     const float2* ml = ml_all + group * gw * ROWS;
 
     uint32_t qf[NT][KSTEPS][2];                             // Q of row n (this lane: n = g4) as B operand
+    // m is the largest score less kPagedShift; what leaves the warp as l and o is without the factor 2^15 that comes of it
     float m[NT][2], l[NT][2], o[NT][KSTEPS][4], vref = 0.f, vmax = 0.f;
     if (lane == 0) s_slot[warp] = 0;                        // a warp that computes nothing is read, and not used
     int slot = 0, u = 0;
@@ -513,12 +518,13 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float top = m[nt][e];
+                    float top = -INFINITY;
 #pragma unroll
                     for (int sl = 0; sl < SLABS; ++sl) top = fmaxf(top, fmaxf(s[sl][nt][e], s[sl][nt][e + 2]));
                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+                    top = fmaxf(m[nt][e], __fadd_ru(top, -kPagedShift));     // rounded up: no weight is above 2^15, whatever the scores
                     const float ref = top == -INFINITY ? 0.f : top;
                     alpha[nt][e] = fast_exp2(m[nt][e] - ref);
                     m[nt][e] = top;
@@ -700,7 +706,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                 x += __shfl_xor_sync(~0u, x, 4);
                 x += __shfl_xor_sync(~0u, x, 8);
                 x += __shfl_xor_sync(~0u, x, 16);
-                if (g4 == 0) ml_all[warp * ROWS + nt * 8 + t4 * 2 + e] = make_float2(m[nt][e], x);
+                if (g4 == 0) ml_all[warp * ROWS + nt * 8 + t4 * 2 + e] = make_float2(m[nt][e], x * kPagedUnshift);
             }
         auto put = [&](int row, int col, float2 x, float top, float denom) {
             const int r = at.rb * ROWS + row, j = __umulhi(2 * r, a.group_inv);
@@ -709,7 +715,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             x = denom == 0.f ? make_float2(0.f, 0.f) : make_float2(x.x * inv, x.y * inv);
             if (F32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.output) + to * D + col) = x;
             else *reinterpret_cast<uint32_t*>(reinterpret_cast<__half*>(a.output) + to * D + col) = pack_half2(x.x, x.y);
-            if (a.lse && col == 0) a.lse[to] = denom == 0.f ? -INFINITY : (top + __log2f(denom)) * kLn2;
+            if (a.lse && col == 0) a.lse[to] = denom == 0.f ? -INFINITY : (top + kPagedShift + __log2f(denom)) * kLn2;
         };
         // Through the slots that the warps read last.  Columns of rows 2i, 2i + 1 are xored with 8 i: other banks.  A warp that
         // had no unit of the segment has no such slot, and no weight.
@@ -723,13 +729,13 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                     const float (&c)[4] = o[nt][j];
                     if (kScaled) {
                         float* at_ = to + nt * 8 * D + ((j * 16 + 2 * g4) ^ (t4 * 8));
-                        *reinterpret_cast<float2*>(at_) = make_float2(c[0] * gain, c[2] * gain);
-                        *reinterpret_cast<float2*>(at_ + D) = make_float2(c[1] * gain, c[3] * gain);
+                        *reinterpret_cast<float2*>(at_) = make_float2(c[0] * kPagedUnshift * gain, c[2] * kPagedUnshift * gain);
+                        *reinterpret_cast<float2*>(at_ + D) = make_float2(c[1] * kPagedUnshift * gain, c[3] * kPagedUnshift * gain);
                     } else {
                         float* at_ = to + nt * 8 * D + ((j * 16 + g4) ^ (t4 * 8));
                         float* at8 = to + nt * 8 * D + ((j * 16 + 8 + g4) ^ (t4 * 8));
-                        at_[0] = c[0]; at8[0] = c[2];
-                        at_[D] = c[1]; at8[D] = c[3];
+                        at_[0] = c[0] * kPagedUnshift; at8[0] = c[2] * kPagedUnshift;
+                        at_[D] = c[1] * kPagedUnshift; at8[D] = c[3] * kPagedUnshift;
                     }
                 }
         }
