@@ -87,3 +87,30 @@ def test_a_few_positions_outweigh_all_others(dev, kind, case):
         assert (off <= limit).all(), (f32, np.unravel_index(np.argmax(off - limit), off.shape), (off / limit).max(), np.linalg.norm(off) / np.linalg.norm(ref))
         # the logarithm's own two roundings, a sum of weights off by 8 roundings of `reach` and 2^-20, and its additions
         assert (np.abs(lse - ref_lse) <= 2.0 ** -20 * bound[1] + 2.0 ** -16 + 2.0 ** -22 * np.abs(ref_lse)).all()
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("D,page", [(64, 64), (64, 128), (128, 32), (256, 16), (64, 16)])
+def test_v_scales_of_all_kinds_in_units_of_one_page(dev, kind, D, page):
+    """Zero, negative, huge and tiny V scales beside ordinary ones, from page to page of a sequence: the unit of the sums
+    changes between the quick way and the careful one."""
+    rng = np.random.default_rng([D, page])
+    heads = Hq, H, _ = (4, 2, D)
+    palettes = [[0, 1, -1], [1e31, -1e31, 1e28], [2.0 ** -110, 0, 2.0 ** -105], [1, 1e-13, 0], [1, 1e31, 0, -1, 1e-30], [-1, -2], [0], [1, 1, 1, 0],
+                [2.0 ** 101, 2.0 ** 99, 2.0 ** 98]]
+    lengths = rng.integers(1, 1500, size=81)
+    table, pages = table_of(rng, lengths, page)
+    pools, scales = [], []
+    for _ in range(2):
+        x, s = stored(rng.standard_normal((pages, H, page, D), dtype=np.float32), kind)
+        pools.append(x)
+        scales.append(s)
+    for b, n in enumerate(lengths):
+        for p in table[b, :-(-int(n) // page)]:
+            scales[1][p] = rng.choice(np.array(palettes[b % len(palettes)], dtype=np.float32), size=H)
+    q = rng.standard_normal((len(lengths), 1, Hq, D), dtype=np.float32).astype(np.float16)
+    out, _ = attend(dev, kind, heads, page, table, lengths, pools, scales, q, True)
+    ref, _, (mean, reach, floor) = definition(kind, heads, table, lengths, pools, scales, q)
+    most = tolerance((mean, reach, floor * 2.0 ** -14), ref, D, True) + 2.0 ** -16 * mean
+    off = np.abs(out - ref)
+    assert (off <= most).all(), (np.unravel_index(np.argmax(off - most), off.shape), (off / np.where(most > 0, most, 1)).max())
