@@ -378,7 +378,8 @@ int vteb_paged_append(const vteb_paged_cache_t* cache, const vteb_paged_append_t
  * q and output [batch, query_tokens, num_q_heads, head_dim] contiguous, q fp16, output fp16 or fp32 (out_is_f32); query
  * token i of sequence b sees positions 0..kv_offsets[b] - query_tokens + 1 + i.  A row that sees nothing is zero, and its
  * lse (fp32[batch, query_tokens, num_q_heads], natural log, may be null) -infinity.  Positions that a row does not see do
- * not reach it, whatever they hold.  The result is the same bits for the same inputs.
+ * not reach it, whatever they hold.  An infinite V (fp16 pages) stays infinite in the rows that see it, unless its weight
+ * is below 2^-126 of the largest.  The result is the same bits for the same inputs.
  * workspace: vteb_paged_attention_workspace bytes, 256-byte aligned, zeroed before its first use (each call leaves it ready
  * for the next).  Calls that share one must not overlap on the GPU, whatever their shapes.
  * status as above, and 1 where a bounded wait ran out; the rows of a sequence with a table entry outside the pool are NaN,

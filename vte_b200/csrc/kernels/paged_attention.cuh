@@ -121,6 +121,18 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
     return y;
 }
 
+__device__ __forceinline__ uint32_t pack_half2_down(float x, float y) {      // towards zero
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %2, %1;" : "=r"(r) : "f"(x), "f"(y));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t above_zero(uint32_t x) {     // both halves, at least 2^-24; NaN stays NaN
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x00010001u));
+    return r;
+}
+
 // Four 8-bit values to fp16, exactly: lo = values 0 and 1 of the word (2 and 3 with them in hi), or with `PAIRS` 0 and 2
 // (1 and 3), which is how ldmatrix.trans leaves two positions of two channels.
 template <int KIND, bool PAIRS>
@@ -653,11 +665,15 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float x = s[sl][nt][2 * e], y = s[sl][nt][2 * e + 1];
-                        const uint32_t h = pack_half2(x, y);
+                        // An infinite V stays infinite only under weights above zero: those of 16-bit pages are no less than fp16's
+                        // least, 2^-39 of the largest, and the low part is what a high one rounded down leaves.  (Rows that not all
+                        // see are zeros by now.)
+                        const uint32_t h = kScaled ? pack_half2(x, y) : above_zero(F32 ? pack_half2_down(x, y) : pack_half2(x, y));
                         p[nt][e] = transpose_8x8(h);
                         if (F32) {
                             const float2 back = unpack_half2(h);
-                            pl[nt][e] = transpose_8x8(pack_half2(x - back.x, y - back.y));
+                            const uint32_t low = pack_half2(x - back.x, y - back.y);
+                            pl[nt][e] = transpose_8x8(kScaled ? low : above_zero(low));
                         }
                     }
                 const int box = (sl * 16) >> a.box_log2;
@@ -817,20 +833,24 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                         float4 v[AHEAD];
 #pragma unroll
                         for (int q = 0; q < AHEAD; ++q) {
-                            const int from = place(start + min(k0 + q, count - 1) * step) * ROWS + row;
-                            y[q] = __ldcg(ml_from + from);
-                            v[q] = __ldcg(reinterpret_cast<const float4*>(a.part_o + from * D + col));
+                            y[q] = make_float2(-INFINITY, 0.f);
+                            v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (k0 + q < count) {
+                                const int from = place(start + (k0 + q) * step) * ROWS + row;
+                                y[q] = __ldcg(ml_from + from);
+                                v[q] = __ldcg(reinterpret_cast<const float4*>(a.part_o + from * D + col));
+                            }
                         }
                         float over = top;
 #pragma unroll
-                        for (int q = 0; q < AHEAD; ++q) over = fmaxf(over, y[q].x);      // (one that is read twice does no harm here)
+                        for (int q = 0; q < AHEAD; ++q) over = fmaxf(over, y[q].x);
                         const float ref = over == -INFINITY ? 0.f : over, old = fast_exp2(top - ref);
                         top = over;
                         denom *= old;
                         x.x *= old; x.y *= old; x.z *= old; x.w *= old;
 #pragma unroll
                         for (int q = 0; q < AHEAD; ++q) {
-                            const float f = k0 + q < count ? fast_exp2(y[q].x - ref) : 0.f;
+                            const float f = fast_exp2(y[q].x - ref);
                             denom += y[q].y * f;
                             x.x += v[q].x * f; x.y += v[q].y * f; x.z += v[q].z * f; x.w += v[q].w * f;
                         }
