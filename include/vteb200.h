@@ -382,8 +382,8 @@ int vteb_paged_append(const vteb_paged_cache_t* cache, const vteb_paged_append_t
  * is below 2^-126 of the largest.  The result is the same bits for the same inputs.
  * workspace: vteb_paged_attention_workspace bytes, 256-byte aligned, zeroed before its first use (each call leaves it ready
  * for the next).  Calls that share one must not overlap on the GPU, whatever their shapes.
- * status as above, and 1 where a bounded wait ran out; the rows of a sequence with a table entry outside the pool are NaN,
- * and a kv_offset beyond the table stands for the table's last position. */
+ * status as above, and 1 where a bounded wait ran out; the rows that this leaves incomplete, and those of a sequence with a
+ * table entry outside the pool, are NaN, and a kv_offset beyond the table stands for the table's last position. */
 typedef struct vteb_paged_attention_t {
     const void* q;
     void* output;

@@ -74,6 +74,7 @@ constexpr int kPagedMaxWorkers = 2;      // of a CTA
 constexpr int kPagedJoin = 8;            // pieces that are merged at once (sixteen: 8,000 positions of 2 x 256-wide fp16 heads 14.8 us instead of 13.8)
 constexpr int kPagedTwoFrom = 4, kPagedTwoBelow = 192, kPagedAligned = 8, kPagedUnitsOfAWarp = 2, kPagedSegmentEnd = 2;
 
+constexpr long long kPagedLandingCycles = 4000000000;      // for copies of a warp that gave up: about two seconds a slot
 constexpr float kPagedShift = 15.f, kPagedUnshift = 0x1p-15f;     // 2^15 is the largest power of two that fp16 has
 
 template <int D, int KIND, int NT>
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 m[nt][0] = m[nt][1] = -INFINITY;
-                l[nt][0] = l[nt][1] = 0.f;
+                l[nt][0] = l[nt][1] = dead && u < at.end ? NAN : 0.f;
                 const int r = at.rb * ROWS + nt * 8 + g4;
                 const int j = __umulhi(2 * r, a.group_inv), g = r - j * a.group;
                 const __half* src = a.q + (((long long)at.b * a.queries + j) * a.num_q_heads + at.head * a.group + g) * D;
@@ -467,9 +468,21 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                     }
             }
             if (kScaled) asm volatile("cp.async.wait_group %0;" ::"n"(NS - 1) : "memory");
-            if (!dead && !mbar_wait_bounded(bars_u + slot * 8, phase, nullptr)) {
+            // Each lane's wait has its own limit: the warp gives up as one, as it has to be whole for what follows.  Rows that it
+            // had a part of are NaN then, it asks for nothing more, and the copies under way land before it goes on, as the slots
+            // are not its own until then: from this slot up to the one that would be filled next.
+            if (!dead && __any_sync(~0u, !mbar_wait_bounded(bars_u + slot * 8, phase, nullptr))) {
                 dead = true;
-                if (a.status) *a.status = kStatusFullTimeout;
+                if (lane == 0 && a.status) *a.status = kStatusFullTimeout;
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                uint32_t under_way = phase;
+                int i = slot;
+                do {
+                    mbar_wait_bounded(bars_u + i * 8, under_way, nullptr, kPagedLandingCycles);
+                    if (++i == NS) { i = 0; under_way ^= 1; }
+                } while (i != fill_slot);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) l[nt][0] = l[nt][1] = NAN;
             }
             __syncwarp();
 
@@ -734,9 +747,9 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             if (a.lse && col == 0) a.lse[to] = denom == 0.f ? -INFINITY : (top + kPagedShift + __log2f(denom)) * kLn2;
         };
         // Through the slots that the warps read last.  Columns of rows 2i, 2i + 1 are xored with 8 i: other banks.  A warp that
-        // had no unit of the segment has no such slot, and no weight.
+        // had no unit of the segment has no such slot, and no weight; one that gave up leaves what is there, under weights of NaN.
         const float gain = kScaled ? vref : 1.f;
-        if (at.first + wi < at.end) {
+        if (at.first + wi < at.end && !dead) {
             float* to = reinterpret_cast<float*>(ring + s_slot[warp] * S::SLOT) + t4 * 2 * D;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
