@@ -46,6 +46,8 @@ class PagedKVCache:
         self.num_pages, self.page_size, self.cache_type = int(num_pages), int(page_size), cache_type
         self._allocator = allocator
         self._owned: list = []
+        self._life = self._life_of_runtime()
+        self._closed = False
         self._workspace, self._workspace_bytes = 0, 0
         given = [_ptr_value(p) for p in (k_pool, v_pool, k_scale, v_scale)]
         if any(given[:2]) != all(given[:2]) or (any(given[2:]) and not given[0]):
@@ -58,7 +60,8 @@ class PagedKVCache:
             raise CudaSafetyError("strides belong to pools of the caller's")
         if len(strides) != 3:
             raise CudaSafetyError(f"strides are (page, token, head), not {strides!r}")
-        if not given[0]:
+        self._owns_pools = not given[0]
+        if self._owns_pools:
             size = self.num_pages * self.num_kv_heads * self.page_size * self.head_dim * (2 if cache_type == "f16" else 1)
             scales = 0 if cache_type == "f16" else self.num_pages * self.num_kv_heads * 4
             try:
@@ -86,6 +89,14 @@ class PagedKVCache:
         self._default_scale = 1.0 / math.sqrt(self.head_dim)
 
     # ------------------------------------------------------------------ memory
+    def _life_of_runtime(self):
+        """What a runtime has from one `initialize` to its `cleanup`, at which all that it allocated is freed."""
+        return getattr(self.hip, '_launch_status', None)
+
+    def _require_pools(self) -> None:
+        if self._owns_pools and (self._closed or self._life is not self._life_of_runtime()):
+            raise CudaSafetyError("the cache or its runtime has been cleaned up: its pools are gone")
+
     def _allocate(self, size: int, tag: str) -> int:
         if self._allocator is not None:
             block = self._allocator.allocate(size, tag, MemoryRegion.SCRATCH if tag == "paged_workspace" else MemoryRegion.KV_CACHE)
@@ -107,7 +118,11 @@ class PagedKVCache:
 
     def reserve(self, batch_size: int, query_tokens: int = 1) -> None:
         """Allocates the workspace of this cache's own, where the one it has does not do.  Not while the stream is captured."""
+        self._require_pools()
         need = self.hip.paged_attention_workspace(self.num_q_heads, self.num_kv_heads, self.head_dim, batch_size, query_tokens)
+        if self._life is not self._life_of_runtime():        # went with the runtime's cleanup
+            self._owned.clear()
+            self._workspace, self._workspace_bytes, self._life = 0, 0, self._life_of_runtime()
         if need > self._workspace_bytes:
             # earlier ones stay until cleanup: a captured step may still name them
             self._workspace = self._allocate(need + 256, "paged_workspace") + 255 & ~255
@@ -129,6 +144,7 @@ class PagedKVCache:
         """New tokens into the pages of their sequences: one a sequence, or `total_tokens` rows cut by `token_starts`
         (int32[batch + 1]; without it the same number each).  The newest token of sequence b goes to position kv_offsets[b].
         `token_strides`: halves between the tokens of k, v, q and q_out where their rows lie in something wider."""
+        self._require_pools()
         a = self._append
         a.k, a.v, a.q, a.q_out = _address(k), _address(v), _address(q), _address(q_out)
         a.block_table, a.kv_offsets, a.token_starts = _address(block_table), _address(kv_offsets), _address(token_starts)
@@ -140,6 +156,7 @@ class PagedKVCache:
                output_f32: bool = False, lse=0, workspace=0, workspace_bytes: int = 0, stream=None) -> None:
         """The newest `query_tokens` tokens of each sequence over its cached positions, causally among themselves.
         `output` like q, fp16 or (`output_f32`) fp32; `lse` optional fp32 [batch, query_tokens, heads]."""
+        self._require_pools()
         a = self._attention
         if workspace:
             a.workspace, a.workspace_bytes = _address(workspace), workspace_bytes
@@ -153,8 +170,10 @@ class PagedKVCache:
         self.hip.paged_attention(self._cache, a, stream)
 
     def cleanup(self) -> None:
-        """Frees what this cache allocated (a runtime that has been cleaned up has done so already)."""
-        if self._allocator is None and not getattr(self.hip, "_initialized", True):
+        """Frees what this cache allocated (a runtime that has been cleaned up has done so already).  A cache with pools of its own
+        refuses calls from then on."""
+        self._closed = True
+        if self._life is not self._life_of_runtime() or (self._allocator is None and not getattr(self.hip, "_initialized", True)):
             self._owned.clear()
         for block in self._owned:
             if self._allocator is not None:
