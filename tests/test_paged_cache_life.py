@@ -1,4 +1,4 @@
-"""`PagedKVCache` after its memory is gone, without a device."""
+"""`PagedKVCache` after its memory is gone, and calls that would drop tokens, without a device."""
 import ctypes
 
 import pytest
@@ -82,3 +82,14 @@ def test_pools_of_the_callers_outlive_a_cleanup():
         again()
     cache.cleanup()
     assert not rt.live
+
+
+def test_ragged_tokens_are_counted():
+    """Without their number, rows behind the first `batch` ones would be left out."""
+    rt = Runtime()
+    cache = PagedKVCache(rt, META, 4, **POOLS)
+    with pytest.raises(CudaSafetyError, match="total_tokens"):
+        cache.append(1, 2, 3, 4, 5, 6, token_starts=AT)
+    assert rt.launches == 0
+    cache.append(1, 2, 3, 4, 5, 6, token_starts=AT, total_tokens=0)
+    assert rt.append["total_tokens"] == 0

@@ -148,6 +148,8 @@ class PagedKVCache:
         a = self._append
         a.k, a.v, a.q, a.q_out = _address(k), _address(v), _address(q), _address(q_out)
         a.block_table, a.kv_offsets, a.token_starts = _address(block_table), _address(kv_offsets), _address(token_starts)
+        if total_tokens is None and a.token_starts:
+            raise CudaSafetyError("token_starts cuts total_tokens rows: their number is missing")
         a.batch, a.max_pages, a.total_tokens = batch, max_pages, batch if total_tokens is None else total_tokens
         a.k_token_stride, a.v_token_stride, a.q_token_stride, a.q_out_token_stride = token_strides or self._default_strides
         self.hip.paged_append(self._cache, a, stream)
