@@ -351,7 +351,7 @@ typedef struct vteb_paged_cache_t {
 int vteb_paged_cache_init(vteb_paged_cache_t* cache);
 
 /* New tokens of each sequence into its pages, K rotated to its positions on the way and, with q, the queries of the same
- * tokens rotated into q_out (which may be q).  k, v [total_tokens, num_kv_heads, head_dim] and q, q_out [total_tokens,
+ * tokens rotated into q_out (which may be q, with q's stride).  k, v [total_tokens, num_kv_heads, head_dim] and q, q_out [total_tokens,
  * num_q_heads, head_dim] fp16, the heads of a token side by side, tokens at the strides given (halves, multiples of 8: k, v
  * and q may be parts of one projection's rows).  The tokens of sequence b are rows token_starts[b] to token_starts[b + 1] -
  * 1 (int32[batch + 1], device), or total_tokens / batch rows each where token_starts is null; the last of them has

@@ -1,10 +1,11 @@
-"""`PagedKVCache` after its memory is gone, and calls that would drop tokens, without a device."""
+"""`PagedKVCache` after its memory is gone, and appends that would drop tokens or race, without a device."""
 import ctypes
 
 import pytest
 
-from tests.test_paged_cache import AT, META, FakeRuntime
+from tests.test_paged_cache import AT, INVALID, META, NOT_INITIALIZED, FakeRuntime, cache_of
 from vte_b200.bridge import CudaSafetyError
+from vte_b200.bridge.cuda_runtime import PagedAppend, load_library
 from vte_b200.core import PagedKVCache
 
 POOLS = {"k_pool": AT, "v_pool": 2 * AT}
@@ -93,3 +94,17 @@ def test_ragged_tokens_are_counted():
     assert rt.launches == 0
     cache.append(1, 2, 3, 4, 5, 6, token_starts=AT, total_tokens=0)
     assert rt.append["total_tokens"] == 0
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"q_out_token_stride": 2048}, INVALID), ({"q_token_stride": 2048}, INVALID), ({"q_token_stride": 2048, "q_out_token_stride": 2048}, NOT_INITIALIZED),
+    ({"q_out_token_stride": 2048, "q_out": 2 * AT}, NOT_INITIALIZED), ({"q_out_token_stride": 2048, "total_tokens": 1, "batch": 1}, NOT_INITIALIZED),
+])
+def test_rotating_in_place_takes_one_stride(built_library, change, code):
+    """With two, a token's rotated row would lie where another token's row is still to be read."""
+    lib = load_library(str(built_library))
+    c = cache_of(ready=1)
+    base = dict(k=AT, v=AT, q=AT, q_out=AT, k_token_stride=256, v_token_stride=256, q_token_stride=1536, q_out_token_stride=1536,
+                block_table=AT, kv_offsets=AT, batch=4, max_pages=3, total_tokens=4, num_q_heads=12, rope_type=-1)
+    a = PagedAppend(**{**base, **change})
+    assert lib.vteb_paged_append(ctypes.byref(c), ctypes.byref(a), None) == code, lib.vteb_last_error_string()

@@ -192,6 +192,8 @@ int vteb_paged_append(const vteb_paged_cache_t* c, const vteb_paged_append_t* a,
         const long long q_row = (long long)a->num_q_heads * D;
         if (a->num_q_heads <= 0 || a->q_token_stride < q_row || a->q_out_token_stride < q_row || a->q_token_stride % 8 || a->q_out_token_stride % 8)
             return report(VTEB_ERR_INVALID_ARGUMENT, "%d query heads, token strides (%lld, %lld): at least %lld halves and multiples of 8", a->num_q_heads, a->q_token_stride, a->q_out_token_stride, q_row);
+        if (a->q == a->q_out && a->q_token_stride != a->q_out_token_stride && a->total_tokens > 1)
+            return report(VTEB_ERR_INVALID_ARGUMENT, "q rotated in place with two token strides (%lld, %lld)", a->q_token_stride, a->q_out_token_stride);
         if ((long long)a->total_tokens * a->num_q_heads > INT_MAX) return report(VTEB_ERR_TOO_LARGE, "%d tokens of %d query heads", a->total_tokens, a->num_q_heads);
     }
     if (a->rope_type < -1 || a->rope_type > 2) return report(VTEB_ERR_INVALID_ARGUMENT, "rope_type %d: -1 (none), 0, 1 or 2", a->rope_type);
