@@ -325,7 +325,8 @@ int vteb_kv_cache_append(const void* k, const void* v, void* k_cache, void* v_ca
  * scale for every page and KV head, of K and of V (k_scale, v_scale fp32[num_pages, num_kv_heads]): a stored value stands
  * for value * scale.  vteb_paged_append keeps the scale at the largest magnitude of the page over 448 (e4m3) or 127
  * (int8): tokens that join a page only ever raise it, and then the page's older tokens are rounded anew under the new
- * scale; the token of a page's first position starts the page afresh.  A value that is not finite makes the scale NaN.
+ * scale; the token of a page's first position starts the page afresh.  (A negative scale that a page came with keeps its
+ * sign.)  A value that is not finite makes the scale NaN.
  * vteb_paged_attention takes any scales.
  *
  * Layout.  Position t of KV head h of page p starts page_stride * p + head_stride * h + token_stride * t values into the

@@ -78,10 +78,10 @@ def append(pools, scales, kind, new, block_table, kv_offsets, token_starts, page
                     old = scale[p, h] if slot else f32(0)
                     amax = np.abs(x[h]).max().astype(f32)               # NaN where one is
                     need = amax / LARGEST[kind] if np.isfinite(amax) else f32(np.nan)
-                    now = f32(np.nan) if np.isnan(need) or np.isnan(old) else max(old, need)
+                    now = f32(np.nan) if np.isnan(need) or np.isnan(old) else max(old, need) if old >= 0 else min(old, -need)
                     inv = f32(0) if now == 0 else f32(1) / now
                     with np.errstate(invalid="ignore"):
-                        if slot and now > old:
+                        if slot and abs(now) > abs(old):
                             pool[p, h, :slot] = narrow(widen(pool[p, h, :slot], kind) * (old / now), kind)
                         pool[p, h, slot:slot + hi - lo + 1] = narrow(x[h].astype(f32) * inv, kind)
                     scale[p, h] = now

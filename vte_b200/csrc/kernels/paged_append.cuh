@@ -4,7 +4,7 @@
 // them in fp32 (each product rounded, as rope_kernel does) and rounds to fp16, which is what a 16-bit page stores.  For
 // 8-bit pages the block then knows the largest magnitude of its tokens, and with the page's scale so far the new scale
 //
-//   need = amax / 448 (e4m3) or / 127 (int8),  scale = max(older tokens in the page ? old scale : 0, need),
+//   need = amax / 448 (e4m3) or / 127 (int8),  scale = max(older tokens in the page ? |old scale| : 0, need) with the old one's sign,
 //   stored = round(x * (1 / scale)),  older tokens, where the scale grew: round(stored * (old / scale)),
 //
 // all in fp32 with correctly rounded divisions, ties to even.  A value that is not finite makes the scale NaN, and with it
@@ -271,7 +271,8 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
         for (int w = 0; w < (T >> 5); ++w) top = max(top, s_top[w]);
         const float amax = __half2float(__ushort_as_half((unsigned short)top));
         const float need = top >= 0x7c00u ? NAN : __fdiv_rn(amax, KIND == 1 ? 448.f : 127.f);
-        const float now = (isnan(need) || isnan(old)) ? NAN : fmaxf(old, need);
+        // a scale that another program gave the page may be negative: it keeps its sign, and grows by magnitude
+        const float top_scale = fmaxf(fabsf(old), need), now = (isnan(need) || isnan(old)) ? NAN : old < 0.f ? -top_scale : top_scale;
         const float inv = now == 0.f ? 0.f : __fdiv_rn(1.f, now);
         if (tid == 0) *scale_at = now;
         unsigned char* pool = (unsigned char*)(is_v ? p.v_pool : p.k_pool) + base;
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
             *reinterpret_cast<uint2*>(dst + t.a) = quantise8<KIND>(xa, inv);
             *reinterpret_cast<uint2*>(dst + t.b) = quantise8<KIND>(xb, inv);
         }
-        if (now > old && slot > 0) {                        // the older tokens of the page under the new scale
+        if (fabsf(now) > fabsf(old) && slot > 0) {                        // the older tokens of the page under the new scale
             const float factor = __fdiv_rn(old, now);
             for (int at = tid; at < slot << tasks_log2; at += T) {
                 uint4* row = reinterpret_cast<uint4*>(pool + (long long)(at >> tasks_log2) * p.token_stride + (at & ((1 << tasks_log2) - 1)) * 16);
