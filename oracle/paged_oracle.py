@@ -79,7 +79,7 @@ def append(pools, scales, kind, new, block_table, kv_offsets, token_starts, page
                     amax = np.abs(x[h]).max().astype(f32)               # NaN where one is
                     need = amax / LARGEST[kind] if np.isfinite(amax) else f32(np.nan)
                     now = f32(np.nan) if np.isnan(need) or np.isnan(old) else max(old, need) if old >= 0 else min(old, -need)
-                    inv = f32(0) if now == 0 else f32(1) / now
+                    inv = f32(0) if now == 0 or (need == 0 and not np.isnan(now)) else f32(1) / now
                     with np.errstate(invalid="ignore"):
                         if slot and abs(now) > abs(old):
                             pool[p, h, :slot] = narrow(widen(pool[p, h, :slot], kind) * (old / now), kind)

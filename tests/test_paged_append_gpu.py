@@ -29,7 +29,7 @@ def half_step(value, scale, kind):
 
 
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
-@pytest.mark.parametrize("given", [[-0.004, -0.5], [0.0, -0.0], [3.0, -3.0, 1e30]], ids=["negative", "zero", "large"])
+@pytest.mark.parametrize("given", [[-0.004, -0.5], [0.0, -0.0], [3.0, -3.0, 1e30], [1e-44, -1e-44, 1e-40]], ids=["negative", "zero", "large", "tiny"])
 def test_append_to_pages_with_scales_of_all_kinds(dev, kind, given):
     """Tokens that raise such a scale, tokens that do not, and tokens of zeros."""
     rng = np.random.default_rng([len(given), len(kind)])

@@ -273,7 +273,8 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
         const float need = top >= 0x7c00u ? NAN : __fdiv_rn(amax, KIND == 1 ? 448.f : 127.f);
         // a scale that another program gave the page may be negative: it keeps its sign, and grows by magnitude
         const float top_scale = fmaxf(fabsf(old), need), now = (isnan(need) || isnan(old)) ? NAN : old < 0.f ? -top_scale : top_scale;
-        const float inv = now == 0.f ? 0.f : __fdiv_rn(1.f, now);
+        // tokens of zeros stay zeros: the reciprocal of a scale below 2^-128 is infinite
+        const float inv = now == 0.f || (need == 0.f && !isnan(now)) ? 0.f : __fdiv_rn(1.f, now);
         if (tid == 0) *scale_at = now;
         unsigned char* pool = (unsigned char*)(is_v ? p.v_pool : p.k_pool) + base;
         for (int at = last; at >= 0 && at < tasks; at -= T) {
