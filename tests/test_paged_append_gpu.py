@@ -69,3 +69,25 @@ def test_append_to_pages_with_scales_of_all_kinds(dev, kind, given):
     orc.append(pools, scales, kind, x, table, offsets, starts, page)
     for pool, scale, (after, now) in zip(pools, scales, got):
         assert np.array_equal(orc.widen(after, kind), orc.widen(pool, kind)) and np.array_equal(now, scale)
+
+
+@pytest.mark.parametrize("end", [-1, -2, -2 ** 31])
+def test_a_padded_rows_tokens_stay_as_they_were(dev, end):
+    """Any negative offset makes all tokens of a row padding, however many there are."""
+    rng = np.random.default_rng(5)
+    heads, page = (4, 2, 64), 16
+    table, pages = table_of(rng, [20, 20], page)
+    pools = [random_pool(rng, "f16", pages, heads, page)[0] for _ in range(2)]
+    cache, ptrs, _ = make_cache(dev, metadata(heads), "f16", page, pools, (None, None))
+    k = rng.standard_normal((10, 2, 64), dtype=np.float32).astype(np.float16)
+    q = rng.standard_normal((10, 4, 64), dtype=np.float32).astype(np.float16)
+    q_out = np.full_like(q, 7)
+    d_q = dev.put(q_out)
+    cache.append(dev.put(k), dev.put(k), dev.put(table), dev.put(np.array([end, 4], dtype=np.int32)), 2, table.shape[1], total_tokens=10,
+                 q=dev.put(q), q_out=d_q)
+    dev.rt.synchronize()
+    after, got = dev.get(d_q, q), [dev.get(p, x) for p, x in zip(ptrs, pools)]
+    cache.cleanup()
+    assert (after[:5] == 7).all() and np.array_equal(after[5:], q[5:])
+    orc.append(pools, (None, None), "f16", (k, k), table, [-1, 4], [0, 5, 10], page)
+    assert all(np.array_equal(a.view(np.uint16), b.view(np.uint16)) for a, b in zip(got, pools))

@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
         } else b = p.each == 1 ? token : token / p.each;
         int first, count;
         token_range(p, b, first, count);
-        const int pos = __ldg(p.kv_offsets + b) - count + 1 + (int)token - first;
-        if ((int)token < first || (int)token >= first + count || pos < 0 || (p.rope_type >= 0 && pos >= p.rope_rows)) return;
+        const int end = __ldg(p.kv_offsets + b), pos = end - (first + count - 1 - (int)token);
+        if ((int)token < first || (int)token >= first + count || end < 0 || pos < 0 || (p.rope_type >= 0 && pos >= p.rope_rows)) return;
         uint4 c = make_uint4(0, 0, 0, 0), s = c;
         if (t.rotated) {
             const long long e = (long long)pos * (p.rope_type == 2 ? p.rotary_dim : D) + t.entry;
