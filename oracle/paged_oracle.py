@@ -41,7 +41,7 @@ def narrow(x, kind):
     if kind == "e4m3":
         return to_e4m3(x)
     with np.errstate(invalid="ignore"):
-        return np.where(np.isnan(x), 0, np.clip(np.rint(x), -127, 127)).astype(np.int8)
+        return np.where(np.isnan(x), 0, np.clip(np.rint(x), -128, 127)).astype(np.int8)
 
 
 def rotate(x, pos, cos, sin, rope_type, rotary_dim):

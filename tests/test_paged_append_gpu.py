@@ -91,3 +91,19 @@ def test_a_padded_rows_tokens_stay_as_they_were(dev, end):
     assert (after[:5] == 7).all() and np.array_equal(after[5:], q[5:])
     orc.append(pools, (None, None), "f16", (k, k), table, [-1, 4], [0, 5, 10], page)
     assert all(np.array_equal(a.view(np.uint16), b.view(np.uint16)) for a, b in zip(got, pools))
+
+
+def test_older_values_keep_the_whole_range_of_int8(dev):
+    """A page that came from elsewhere may hold -128: a scale that grows by less than a half in 128 leaves it so."""
+    heads, page, n = (2, 1, 64), 16, 5
+    pools = [np.full((1, 1, page, 64), x, dtype=np.int8) for x in (-128, 127)]
+    scales = [np.full((1, 1), 1.0, dtype=np.float32) for _ in range(2)]
+    x = np.full((1, 1, 64), 127.25, dtype=np.float16)                # 1.00197 of the old scale: 128 / 1.00197 = 127.75
+    cache, ptrs, sc = make_cache(dev, metadata(heads), "int8", page, pools, scales)
+    cache.append(dev.put(x), dev.put(x), dev.put(np.zeros((1, 1), dtype=np.int32)), dev.put(np.array([n], dtype=np.int32)), 1, 1)
+    dev.rt.synchronize()
+    got, now = [dev.get(p, y) for p, y in zip(ptrs, pools)], [dev.get(p, y) for p, y in zip(sc, scales)]
+    cache.cleanup()
+    for after, scale, value in zip(got, now, (-128, 127)):
+        assert scale[0, 0] == np.float32(127.25) / np.float32(127)
+        assert (after[0, 0, :n] == value).all() and (after[0, 0, n] == 127).all() and (after[0, 0, n + 1:] == value).all()

@@ -97,7 +97,8 @@ __device__ __forceinline__ uint32_t narrow4(float x, float y, float z, float w) 
             : "=r"(r) : "f"(x), "f"(y), "f"(z), "f"(w));
         return r;
     } else {
-        auto one = [](float v) { return (uint32_t)(min(max(__float2int_rn(v), -127), 127)) & 0xffu; };
+        // (-128 only where a page that came from elsewhere held it: x * (1 / scale) rounds to 127 at most)
+        auto one = [](float v) { return (uint32_t)(min(max(__float2int_rn(v), -128), 127)) & 0xffu; };
         return one(x) | one(y) << 8 | one(z) << 16 | one(w) << 24;
     }
 }
