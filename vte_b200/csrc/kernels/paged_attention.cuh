@@ -34,6 +34,7 @@
 
 #include <type_traits>
 
+#include "../paged_partition.h"
 #include "vteb_common.cuh"
 
 namespace vteb {
@@ -67,13 +68,6 @@ struct PagedAttnArgs {
 // of 168 registers or sixteen of 128 do less well (64 sequences of 8 x 64-wide e4m3 heads 103, 114 and 217 us).
 __host__ __device__ constexpr int paged_unit(int row_bytes) { return row_bytes >= 256 ? 16 : 4096 / row_bytes; }
 __host__ __device__ constexpr int paged_warps(int row_bytes) { return row_bytes == 512 ? 6 : 8; }
-constexpr int kPagedMaxWorkers = 2;      // of a CTA
-// Two workers a CTA from one segment on every fourth SM on (four query tokens of 8 sequences of 8 x 128-wide e4m3 heads 30.3 us, 32.4
-// from one an SM on); runs begin with a segment each up to so many units a warp (the same 30.3 us, 31.7 up to 4); units that a
-// warp of a worker has at least (2,000 positions of 2 x 128-wide heads 10.3 us, 11.7 with 3 and 13.0 with 4).
-constexpr int kPagedJoin = 8;            // pieces that are merged at once (sixteen: 8,000 positions of 2 x 256-wide fp16 heads 14.8 us instead of 13.8)
-constexpr int kPagedTwoFrom = 4, kPagedTwoBelow = 192, kPagedAligned = 8, kPagedUnitsOfAWarp = 2, kPagedSegmentEnd = 2;
-
 constexpr long long kPagedLandingCycles = 4000000000;      // for copies of a warp that gave up: about two seconds a slot
 constexpr float kPagedShift = 15.f, kPagedUnshift = 0x1p-15f;     // 2^15 is the largest power of two that fp16 has
 
@@ -166,45 +160,14 @@ __device__ __forceinline__ void group_barrier(int gw, int group) {
     asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(gw * 32) : "memory");
 }
 
-// Where a warp is in its worker's run: unit `u` of a segment, of which units [first, end) are this worker's.
-struct PagedCursor {
-    int b, head, rb, u, first, end, units, len;
-    int left;                                               // what is left of the run from `first` on, ends of segments included
-    int extra;                                              // what the end of a segment counts
+struct PagedLengths {                                       // cached positions of sequence b, no more than its table has room for
+    const PagedAttnArgs& a;
+    __device__ __forceinline__ int operator()(int b) const {
+        const int room = a.max_pages << a.page_log2;        // at most 2^30, checked by the host
+        const int off = __ldg(a.kv_offsets + b);
+        return off < 0 ? 0 : off >= room ? room : off + 1;
+    }
 };
-
-__device__ __forceinline__ int paged_len(const PagedAttnArgs& a, int b) {
-    const int room = a.max_pages << a.page_log2;            // at most 2^30, checked by the host
-    const int off = __ldg(a.kv_offsets + b);
-    return off < 0 ? 0 : off >= room ? room : off + 1;
-}
-
-template <int U>
-__device__ __forceinline__ void cursor_enter(const PagedAttnArgs& a, PagedCursor& c) {   // first sequence at or behind c.b that has units
-    c.len = paged_len(a, c.b);
-    c.units = (c.len + U - 1) / U;
-    while (c.units == 0 && c.b + 1 < a.batch) {
-        c.len = paged_len(a, ++c.b);
-        c.units = (c.len + U - 1) / U;
-    }
-}
-
-template <int U>
-__device__ __forceinline__ bool cursor_next_segment(const PagedAttnArgs& a, PagedCursor& c) {
-    c.left -= (c.end == c.units ? c.units + c.extra : c.end) - c.first;
-    if (c.left <= 0) return false;
-    c.first = 0;
-    if (++c.rb == a.row_blocks) {
-        c.rb = 0;
-        if (++c.head == a.num_kv_heads) {
-            c.head = 0;
-            if (++c.b == a.batch) return false;             // (the run ends with the last segment's end)
-            cursor_enter<U>(a, c);
-        }
-    }
-    c.end = min(c.units, c.left);
-    return c.units > 0;                                     // (no units left: lengths that changed under the launch)
-}
 
 template <int D, int KIND, int NT, bool F32>
 __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_attention_kernel(const __grid_constant__ PagedAttnArgs a)
@@ -243,7 +206,8 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
     const int HR = a.num_kv_heads * a.row_blocks;
 
     // ---- all units, and where this CTA's workers begin ------------------------------------------
-    auto units_of = [&](int b) { return (paged_len(a, b) + U - 1) / U; };
+    const PagedLengths lengths{a};
+    auto units_of = [&](int b) { return (lengths(b) + U - 1) / U; };
     const int per_thread = (a.batch + W * 32 - 1) / (W * 32);
     const int b0 = min(tid * per_thread, a.batch), b1 = min(b0 + per_thread, a.batch);
     int total = 0, lives = 0, mine = 0, upto = 0;
@@ -279,29 +243,14 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
         for (int w = 0; w < W; ++w) lives += s_live[w];
     }
     total *= HR;
-    // Workers of a CTA: two where there are segments for them and these are short, so that one computes while the other merges;
-    // one where few segments would be cut more often for that, or where merges are rare beside units (one and two workers: 64
-    // sequences of 8 x 64-wide heads, 136 units of e4m3 each, 100.1 and 96.7 us, 272 units of fp16 each, 151 and 155;
-    // 100 of 10 to 8,000 positions 94 and 86; one of 32,768 positions 12.8 and 14.9).
-    const int segments = max(lives * HR, 1), grid = gridDim.x;      // (1 where nothing is cached: no worker has a unit then)
-    const int mean = max((total + segments - 1) / segments, 1);
-    const int groups = segments * kPagedTwoFrom >= grid && mean < kPagedTwoBelow ? kPagedMaxWorkers : 1, workers = grid * groups;
-    const int gw = W / groups, group = groups == 1 ? 0 : warp / (W / 2), wi = groups == 1 ? warp : warp % (W / 2);
-    // Units of a worker: an equal share, but not so few that a segment is cut where its warps would have little to do each.
-    // Short runs begin with a segment each: `per` units stand for what is left of one, so that no worker has parts of two.
-    const bool aligned = segments * 2 <= workers && total < workers * gw * kPagedAligned;
-    const int cuts = (mean + kPagedUnitsOfAWarp * gw - 1) / (kPagedUnitsOfAWarp * gw);
-    const int over = !aligned ? workers : a.batch == 1 ? workers / segments * segments : workers - segments;
-    // Long runs count the end of a segment, at which a worker's warps wait for one another, as units too, kPagedSegmentEnd a warp:
-    // else runs of many short segments take half as long again as runs of one (100 sequences of 10 to 8,000 positions of
-    // 8 x 64-wide e4m3 heads 86 us, 124 without; 64 of 1,024 to 16,384 97 and 102).
-    const int extra = aligned ? 0 : kPagedSegmentEnd * gw;
-    const int per = max((total + extra * lives * HR + over - 1) / over, (mean + cuts - 1) / cuts);
-    auto room_of = [&](int units) { return units == 0 ? 0 : aligned ? (units + per - 1) / per * per : units + extra; };
-    if (a.batch == 1) total = lives ? room_of(mean) * segments : 0;
+    const int grid = gridDim.x;
+    const PagedDeal deal = paged_deal(total, lives, HR, a.batch, grid, W);
+    const int groups = deal.groups, gw = deal.gw, per = deal.per;
+    const int group = groups == 1 ? 0 : warp / (W / 2), wi = groups == 1 ? warp : warp % (W / 2);
+    if (a.batch == 1) total = lives ? deal.room_of(deal.mean) * HR : 0;
     else {
         __syncthreads();                                    // s_scan is written anew
-        scan([&](int b) { return room_of(units_of(b)); });
+        scan([&](int b) { return deal.room_of(units_of(b)); });
         total *= HR;
     }
     const int worker = blockIdx.x * groups + group;
@@ -312,7 +261,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             if (at >= (upto - mine) * HR && at < upto * HR) {
                 int rest = at - (upto - mine) * HR, b = b0;
                 for (; b < b1; ++b) {
-                    const int n = room_of(units_of(b)) * HR;
+                    const int n = deal.room_of(units_of(b)) * HR;
                     if (rest < n) break;
                     rest -= n;
                 }
@@ -324,23 +273,14 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
     }
 
     if (lo < total) {
-    PagedCursor at;                                         // what this warp computes
-    {
-        at.b = a.batch > 1 ? s_start_b[group] : 0;
-        cursor_enter<U>(a, at);
-        const int rest = a.batch > 1 ? s_start_rest[group] : lo, room = room_of(at.units), hr = rest / room;
-        at.extra = extra;
-        at.first = rest - hr * room;
-        at.left = min(per, (aligned ? at.units - at.first : total - lo));
-        at.head = a.row_blocks == 1 ? hr : hr / a.row_blocks;
-        at.rb = a.row_blocks == 1 ? 0 : hr - at.head * a.row_blocks;
-        at.end = min(at.units, at.first + at.left);
-    }
+    PagedCursor at = paged_begin<U>(deal, lengths, a.batch > 1 ? s_start_b[group] : 0, a.batch > 1 ? s_start_rest[group] : lo, total - lo,
+                                    a.batch, a.row_blocks);         // what this warp computes
+    const auto next_segment = [&](PagedCursor& c) { return paged_next<U>(lengths, c, a.batch, a.num_kv_heads, a.row_blocks); };
     const int hi = lo + at.left;
     bool any = true;
     if (at.first >= at.units) {                             // the run begins within the end of a segment
         at.end = at.units;
-        any = cursor_next_segment<U>(a, at);
+        any = next_segment(at);
     }
     if (any) {
     // ---- the ring: tables, scales, K and V on their way ----------------------------------------------
@@ -357,7 +297,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             cur = nxt;
             taken = 0;
             nxt.n = 0;
-            while (more && ahead.u >= ahead.end) { more = cursor_next_segment<U>(a, ahead); ahead.u = ahead.first + wi; }
+            while (more && ahead.u >= ahead.end) { more = next_segment(ahead); ahead.u = ahead.first + wi; }
             if (!more) continue;
             nxt.n = min(32 >> box_lanes, (ahead.end - ahead.u + gw - 1) / gw);
             nxt.u = ahead.u;
@@ -726,7 +666,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
         const bool entire = at.first == 0 && at.end == at.units;
         const bool has_first = at.left == hi - lo;
         const int rows_here = min(ROWS, rows_all - at.rb * ROWS);
-        const int piece = 2 * worker + (has_first ? 0 : 1);               // where a cut segment's piece goes
+        const int piece = paged_piece(worker, has_first);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -806,21 +746,14 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             }
         }
         if (!entire) {
-            // the workers whose runs hold units of this segment
-            const int begin = hi - at.left - at.first;      // its first unit, of all
-            const int w0 = begin / per, w1 = (begin + at.units - 1) / per, n = w1 - w0 + 1;
-            const int p0 = 2 * w0 + (w0 * per == begin ? 0 : 1);
-            auto place = [&](int k) { return k == 0 ? p0 : 2 * (w0 + k); };     // of a piece
-            // Whoever comes last of up to kPagedJoin consecutive pieces merges those in place, and whoever comes last of these merges
-            // them: the many pieces of a long segment are read by several SMs, most of them ahead of the last piece.
-            const int join = n <= kPagedJoin ? n : n <= kPagedJoin * kPagedJoin ? kPagedJoin : (n + kPagedJoin - 1) / kPagedJoin;
-            const int mine_at = (worker - w0) / join * join;
+            const PagedCut cut = paged_cut(hi - at.left - at.first, at.units, per);
+            const int mine_at = cut.start(worker);
 #pragma unroll 1
             for (int level = 0; level < 2; ++level) {
-                const int step = level ? join : 1, start = level ? 0 : mine_at;
-                const int count = level ? (n + join - 1) / join : min(join, n - start);
-                const bool done = level || join == n;
-                int* counter = a.counters + (level ? 2 * kPagedMaxWorkers * grid : 0) + place(start);
+                const int step = level ? cut.join : 1, start = level ? 0 : mine_at;
+                const int count = cut.count(level, start);
+                const bool done = level || cut.join == cut.n;
+                int* counter = a.counters + (level ? 2 * kPagedMaxWorkers * grid : 0) + cut.place(start);
                 group_barrier(gw, group);
                 if (gt == 0) {
                     __threadfence();                        // for the whole worker: its stores are in front of the barrier
@@ -849,7 +782,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                             y[q] = make_float2(-INFINITY, 0.f);
                             v[q] = make_float4(0.f, 0.f, 0.f, 0.f);
                             if (k0 + q < count) {
-                                const int from = place(start + (k0 + q) * step) * ROWS + row;
+                                const int from = cut.place(start + (k0 + q) * step) * ROWS + row;
                                 y[q] = __ldcg(ml_from + from);
                                 v[q] = __ldcg(reinterpret_cast<const float4*>(a.part_o + from * D + col));
                             }
@@ -872,7 +805,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                         put(row, col, make_float2(x.x, x.y), top, denom);
                         put(row, col + 2, make_float2(x.z, x.w), top, denom);
                     } else {                                // only this thread reads what it overwrites
-                        const int to = place(start) * ROWS + row;
+                        const int to = cut.place(start) * ROWS + row;
                         *reinterpret_cast<float4*>(a.part_o + to * D + col) = x;
                         if (col == 0) reinterpret_cast<float2*>(a.part_ml2)[to] = make_float2(top, denom);
                     }
@@ -880,7 +813,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                 if (done) break;
             }
         }
-        if (!cursor_next_segment<U>(a, at)) break;
+        if (!next_segment(at)) break;
         fresh = true;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");             // the slot's next copies come behind these accesses
         group_barrier(gw, group);                           // what was merged has been read
