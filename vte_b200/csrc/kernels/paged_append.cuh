@@ -10,8 +10,9 @@
 // all in fp32 with correctly rounded divisions, ties to even.  A value that is not finite makes the scale NaN, and with it
 // every result that reads the page.  Blocks behind those of K and V rotate Q.
 //
-// Bound by bytes and instructions for prompts (each value is read once, for 8-bit pages a second time from L1 or L2, and written
-// once), by latency for single tokens.
+// Bound by bytes on their way for prompts (each value is read once, for 8-bit pages a second time from L1 or L2, and written
+// once: a prompt into e4m3 pages fills 61 % of the issue slots, chunks into int8 pages 67 %, and the warps wait for loads), by latency
+// for single tokens: 1.9 us in fp16 and 2.4 in e4m3 pages, a launch behind another in a graph.
 #pragma once
 
 #include "vteb_common.cuh"
@@ -131,8 +132,9 @@ __device__ __forceinline__ uint2 quantise8(uint4 x, float inv) {
 
 // KIND 0: fp16 pages, 1: e4m3, 2: int8.  One 16-channel task of K and V a thread at a time and two of Q, whose position, table rows
 // and conversions are then looked up once; 8-bit pages read all but a thread's last task a second time, from L1 or L2, rather than
-// hold them.  Registers without spills come before more blocks an SM.  A 32,768-token prompt of 12 query and 2 KV heads of 128 into
-// e4m3 pages: 46.5 us; 54.5 with seven blocks of spilling threads, 48.4 with one task of Q a thread, 52 with four.
+// hold them.  Registers with next to no spills (8 bytes in the fp16 build) come before more blocks an SM.  A 32,768-token prompt of 12
+// query and 2 KV heads of 128 into e4m3 pages: 48.3 us, 52.7 with one task of Q a thread (prompts into fp16 pages 36.9 and 39.7);
+// when blocks and tasks were chosen, side by side, 46.5, with seven blocks of spilling threads 54.5 and with four tasks 52.
 template <int KIND>
 __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_constant__ PagedAppendArgs p)
 {

@@ -27,9 +27,10 @@
 // (m, l, o) pieces in the workspace, and the last worker to arrive merges them in worker order: results do not depend on
 // who is last, and no block waits for another.
 //
-// Bound by bytes on long or many sequences (from 16.8 to 537 MB of e4m3 6.1 TB/s, 64 ragged fp16 sequences 90 % of the copy
-// bandwidth with start and end), by latency on short ones: 512 positions take 7.9 us, of which the chain of offset, table
-// entry, tile, two units a warp and merge is all but the launch.
+// Bound by bytes on long or many sequences (64 ragged ones of 8 x 64-wide heads with start and end: fp16 93 % of the copy
+// bandwidth, e4m3 79 to 84 from machine to machine), by latency on short ones: 512 positions take 7.8 us, of which the chain of
+// offset, table entry, tile, two units a warp and merge is all but the launch.  With 16 rows a segment a warp's products,
+// conversions and softmax wait for one another: two warps a scheduler fill 40 % of its issue slots.
 #pragma once
 
 #include <type_traits>
@@ -65,7 +66,7 @@ struct PagedAttnArgs {
 
 // Positions of a unit (4 or 8 KB of K, and as much of V) and warps of a CTA, so that the rings (192 KB of an SM's 227) hold at
 // least two units a warp.  Few warps with many registers: a warp's own loads, conversions and products overlap, which twelve
-// of 168 registers or sixteen of 128 do less well (64 sequences of 8 x 64-wide e4m3 heads 103, 114 and 217 us).
+// of 168 registers or sixteen of 128 do less well (64 sequences of 8 x 64-wide e4m3 heads, side by side: 103, 114 and 217 us).
 __host__ __device__ constexpr int paged_unit(int row_bytes) { return row_bytes >= 256 ? 16 : 4096 / row_bytes; }
 __host__ __device__ constexpr int paged_warps(int row_bytes) { return row_bytes == 512 ? 6 : 8; }
 constexpr long long kPagedLandingCycles = 4000000000;      // for copies of a warp that gave up: about two seconds a slot

@@ -12,8 +12,8 @@ namespace vteb {
 
 constexpr int kPagedMaxWorkers = 2;      // of a CTA
 // Two workers a CTA from one segment on every fourth SM on (four query tokens of 8 sequences of 8 x 128-wide e4m3 heads 30.3 us, 32.4
-// from one an SM on); runs begin with a segment each up to so many units a warp (the same 30.3 us, 31.7 up to 4); units that a
-// warp of a worker has at least (2,000 positions of 2 x 128-wide heads 10.3 us, 11.7 with 3 and 13.0 with 4).
+// from one an SM on: that case alone); runs begin with a segment each up to so many units a warp (the same 30.3 us, 31.7 up to 4);
+// units that a warp of a worker has at least (2,000 positions of 2 x 128-wide heads 10.3 us, 11.7 with 3 and 13.0 with 4).
 constexpr int kPagedJoin = 8;            // pieces that are merged at once (sixteen: 8,000 positions of 2 x 256-wide fp16 heads 14.8 us instead of 13.8)
 constexpr int kPagedTwoFrom = 4, kPagedTwoBelow = 192, kPagedAligned = 8, kPagedUnitsOfAWarp = 2, kPagedSegmentEnd = 2;
 
@@ -35,7 +35,9 @@ VTEB_PAGED_HD PagedDeal paged_deal(int units, int lives, int head_rows, int batc
     // Workers of a CTA: two where there are segments for them and these are short, so that one computes while the other merges;
     // one where few segments would be cut more often for that, or where merges are rare beside units (one and two workers: 64
     // sequences of 8 x 64-wide heads, 136 units of e4m3 each, 100.1 and 96.7 us, 272 units of fp16 each, 151 and 155;
-    // 100 of 10 to 8,000 positions 94 and 86; one of 32,768 positions 12.8 and 14.9).
+    // 100 of 10 to 8,000 positions 94 and 86; one of 32,768 positions 12.8 and 14.9).  Over eight lengths, one token a sequence:
+    // 512 e4m3 segments gain by two 7 % at 24 units a segment, 3 at 192 and 2 at 512, 512 fp16 ones 6 % at 24, and lose
+    // 1 to 3 from 96 on; 32 to 128 segments mostly lose, 1 to 5 %, at 48 units up to 15.  The limits lie between these.
     const int segments = paged_max(lives * head_rows, 1);         // (1 where nothing is cached: no worker has a unit then)
     d.mean = paged_max((units + segments - 1) / segments, 1);
     d.groups = segments * kPagedTwoFrom >= grid && d.mean < kPagedTwoBelow ? kPagedMaxWorkers : 1;
