@@ -80,7 +80,7 @@ __device__ __forceinline__ void rotate_task(const ChannelTask& t, uint4& xa, uin
 // The token range of sequence b, and the position of its first token.
 __device__ __forceinline__ void token_range(const PagedAppendArgs& p, int b, int& first, int& count) {
     if (p.token_starts) {
-        const int lo = __ldg(p.token_starts + b), hi = __ldg(p.token_starts + b + 1);
+        const int lo = p.token_starts[b], hi = p.token_starts[b + 1];
         first = min(max(lo, 0), p.total_tokens);
         count = max(min(hi, p.total_tokens) - first, 0);
     } else {
@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
 {
     const int D = 1 << p.dim_log2, tasks_log2 = p.dim_log2 - 4, P = 1 << p.page_log2;
     const int tid = threadIdx.x, T = blockDim.x;
-    // nothing of the launches in front is touched before this; the launch behind may start when they are complete
+    // Nothing of the launches in front is touched before this; the launch behind may start when they are complete.  Ordinary loads
+    // throughout: a non-coherent one may be moved ahead of the wait, and is not for what is written while the block is there.
     grid_dependency_wait();
     grid_launch_dependents();
     if ((int)blockIdx.x >= p.kv_blocks) {                   // ---- Q
@@ -158,18 +159,18 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
         int b;
         if (p.token_starts) {
             int lo = 0, hi = p.batch;                   // the last sequence that starts at or before the token
-            while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (__ldg(p.token_starts + mid) <= (int)token) lo = mid; else hi = mid; }
+            while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (p.token_starts[mid] <= (int)token) lo = mid; else hi = mid; }
             b = lo;
         } else b = p.each == 1 ? token : token / p.each;
         int first, count;
         token_range(p, b, first, count);
-        const int end = __ldg(p.kv_offsets + b), pos = end - (first + count - 1 - (int)token);
+        const int end = p.kv_offsets[b], pos = end - (first + count - 1 - (int)token);
         if ((int)token < first || (int)token >= first + count || end < 0 || pos < 0 || (p.rope_type >= 0 && pos >= p.rope_rows)) return;
         uint4 c = make_uint4(0, 0, 0, 0), s = c;
         if (t.rotated) {
             const long long e = (long long)pos * (p.rope_type == 2 ? p.rotary_dim : D) + t.entry;
-            c = __ldg(reinterpret_cast<const uint4*>(p.cos_table + e));
-            s = __ldg(reinterpret_cast<const uint4*>(p.sin_table + e));
+            c = *reinterpret_cast<const uint4*>(p.cos_table + e);
+            s = *reinterpret_cast<const uint4*>(p.sin_table + e);
         }
         __half* dst = p.q_out + token * p.q_out_stride + head * D;
 #pragma unroll 1
@@ -194,9 +195,9 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
     if (p.token_starts) {
         // pages of sequence b: slots token_starts[b] / P + 2 b on, as n tokens touch at most n / P + 2 pages
         int lo = 0, hi = p.batch;
-        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if ((max(__ldg(p.token_starts + mid), 0) >> p.page_log2) + 2 * mid <= x) lo = mid; else hi = mid; }
+        while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if ((max(p.token_starts[mid], 0) >> p.page_log2) + 2 * mid <= x) lo = mid; else hi = mid; }
         b = lo;
-        chunk = x - ((max(__ldg(p.token_starts + b), 0) >> p.page_log2) + 2 * b);
+        chunk = x - ((max(p.token_starts[b], 0) >> p.page_log2) + 2 * b);
     } else {
         const int per = (p.each >> p.page_log2) + 2;
         b = p.each == 1 ? x : x / per;
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
     }
     int first, count;
     token_range(p, b, first, count);
-    const int end = __ldg(p.kv_offsets + b);
+    const int end = p.kv_offsets[b];
     if (count == 0 || end < 0 || chunk < 0) return;
     const int begin = max(end - count + 1, 0);              // tokens at negative positions are padding
     const int nth = (begin >> p.page_log2) + chunk;
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
         hi = p.rope_rows - 1;
         if (lo > hi) return;
     }
-    const int page = __ldg(p.block_table + (long long)b * p.max_pages + nth);
+    const int page = p.block_table[(long long)b * p.max_pages + nth];
     if ((unsigned)page >= (unsigned)p.num_pages) {
         if (tid == 0 && p.status) *p.status = 5;
         return;
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(256, 5) paged_append_kernel(const __grid_const
         xb = *reinterpret_cast<const uint4*>(row + t.b);
         if (t.rotated) {
             const long long e = (long long)(lo + tk) * (rope == 2 ? p.rotary_dim : D) + t.entry;
-            rotate_task(t, xa, xb, __ldg(reinterpret_cast<const uint4*>(p.cos_table + e)), __ldg(reinterpret_cast<const uint4*>(p.sin_table + e)));
+            rotate_task(t, xa, xb, *reinterpret_cast<const uint4*>(p.cos_table + e), *reinterpret_cast<const uint4*>(p.sin_table + e));
         }
         return tk;
     };

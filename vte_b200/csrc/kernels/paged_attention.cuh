@@ -165,7 +165,7 @@ struct PagedLengths {                                       // cached positions 
     const PagedAttnArgs& a;
     __device__ __forceinline__ int operator()(int b) const {
         const int room = a.max_pages << a.page_log2;        // at most 2^30, checked by the host
-        const int off = __ldg(a.kv_offsets + b);
+        const int off = a.kv_offsets[b];
         return off < 0 ? 0 : off >= room ? room : off + 1;
     }
 };
@@ -198,7 +198,8 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             asm volatile("prefetch.tensormap [%0];" ::"l"(&a.v_map) : "memory");
         }
     }
-    // nothing of the launches in front is touched before this; the launch behind may start when they are complete
+    // Nothing of the launches in front is touched before this; the launch behind may start when they are complete.  Ordinary loads
+    // throughout: a non-coherent one may be moved ahead of the wait, and is not for what is written while the block is there.
     grid_dependency_wait();
     grid_launch_dependents();
 
@@ -306,7 +307,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
             nxt.head = ahead.head;
             const int k = lane >> box_lanes;
             const int pos = (ahead.u + k * gw) * U + ((lane & (boxes - 1)) << a.box_log2);
-            nxt.page = k < nxt.n && pos < ahead.len ? __ldg(a.block_table + (long long)ahead.b * a.max_pages + (pos >> a.page_log2)) : 0;
+            nxt.page = k < nxt.n && pos < ahead.len ? a.block_table[(long long)ahead.b * a.max_pages + (pos >> a.page_log2)] : 0;
             ahead.u += nxt.n * gw;
         }
         if (taken < cur.n) {
@@ -382,11 +383,11 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
                     qf[nt][ks][0] = qf[nt][ks][1] = 0;
                     if (r < rows_all) {
                         if (kScaled) {
-                            const uint2 x = __ldg(reinterpret_cast<const uint2*>(src + ks * 16 + t4 * 4));
+                            const uint2 x = *reinterpret_cast<const uint2*>(src + ks * 16 + t4 * 4);
                             qf[nt][ks][0] = x.x; qf[nt][ks][1] = x.y;
                         } else {
-                            qf[nt][ks][0] = __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + t4 * 2));
-                            qf[nt][ks][1] = __ldg(reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + t4 * 2));
+                            qf[nt][ks][0] = *reinterpret_cast<const uint32_t*>(src + ks * 16 + t4 * 2);
+                            qf[nt][ks][1] = *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + t4 * 2);
                         }
                     }
                 }
@@ -827,7 +828,7 @@ __global__ void __launch_bounds__(PagedShape<D, KIND, NT>::W * 32, 1) paged_atte
     // ---- rows of sequences without positions; positions that no table holds -------------------------------
     if (total > 0 && lives == a.batch && a.status == nullptr) return;
     for (int b = blockIdx.x * W + warp; b < a.batch; b += grid * W) {
-        const int off = __ldg(a.kv_offsets + b);
+        const int off = a.kv_offsets[b];
         if (lane == 0 && a.status && off >= (a.max_pages << a.page_log2)) *a.status = kStatusBadPosition;
         if (off >= 0) continue;
         const int rows = a.num_q_heads * a.queries;
